@@ -286,6 +286,102 @@ typedef struct {
 mxfa_status mxfa_gemm(const mxfa_gemm_params *p, const uint8_t *a, const uint8_t *a_sc,
                       const uint8_t *b, const uint8_t *b_sc, void *c, void *stream);
 
+/* ---- 4-bit KV cache ----
+ *
+ * K and V as E2M1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign: OCP MXFP4) in blocks of 32 along the head
+ * dimension of one token, one E8M0 scale to a block: 4.25 bits per element, half of the MXFP8
+ * cache's.  A token is quantized by itself, so no fp32 tail is kept, and it can be written at any
+ * position, again (a rejected draft's place), and for each sequence at its own.  No counterpart in the
+ * reference (it has no cache).
+ *   codes  [B][Hkv][max_len][D/2]             element 2i of a token in the low four bits of byte i, 2i + 1
+ *                                             in the high ones (0-7 the values above, 8-15 negated)
+ *   scales [B][Hkv][max_len/32][4][D/32][8]   token t of a group of 32 at [t % 4][block][2 * (t / 4 % 4) +
+ *                                             t / 16]: the order in which the attention reads them
+ * Rule: e = floor(log2(max |x| of the block)) - 2, limited to -127 .. 125, scale code e + 127; element code
+ * = x / 2^e to the nearest value, half to even, 6 from 5 up.  NaN elements count as 0, infinite ones
+ * become 6 * 2^125 of their sign; -0 keeps its sign.  What is not written is never looked at: codes
+ * and scales of tokens that no query may see can hold anything. */
+
+typedef struct {
+  int32_t batch, num_kv_heads;
+  int32_t head_dim;                         /* multiple of 32                                 */
+  int32_t max_len;                          /* cache capacity in tokens, multiple of 32       */
+} mxfa_kv4_shape;
+
+/* Elements from one batch, head and token to the next of rows of head_dim contiguous elements, e.g. of K
+ * inside the rows of a fused projection's output; every row 16-byte aligned.  NULL or all 0:
+ * dense [batch][head][token][head_dim]. */
+typedef struct {
+  int64_t batch, head, token;
+} mxfa_strides;
+
+/* Write n_new tokens of every sequence: token t of sequence b to position pos[b] + t (pos [B] int32 on the
+ * device; NULL: pos0 + t for every sequence).  counts [B] (device, or NULL: n_new): of sequence b only
+ * the first counts[b] tokens are written (prompts padded to one length).  Positions outside the cache
+ * are skipped (with pos NULL they are MXFA_ERR_INVALID_ARG).  Nothing else in the cache changes.  k_new,
+ * v_new: rows as strides say, fp32 or bf16 (x_fmt, mxfa_c_fmt). */
+mxfa_status mxfa_kv4_append(const mxfa_kv4_shape *c, int32_t x_fmt, const void *k_new, const mxfa_strides *k_strides,
+                            const void *v_new, const mxfa_strides *v_strides, const int32_t *pos, int32_t pos0,
+                            const int32_t *counts, int32_t n_new, uint8_t *k_cache, uint8_t *k_sc, uint8_t *v_cache,
+                            uint8_t *v_sc, void *stream);
+
+/* The values of n tokens of every sequence, from position pos[b] (or pos0) on, exact in bf16 and fp32:
+ * [B][Hkv][n][D] rows as strides say.  Tokens outside the cache read as 0 (with pos NULL they are
+ * MXFA_ERR_INVALID_ARG). */
+mxfa_status mxfa_kv4_read(const mxfa_kv4_shape *c, int32_t x_fmt, const uint8_t *k_cache, const uint8_t *k_sc,
+                          const uint8_t *v_cache, const uint8_t *v_sc, const int32_t *pos, int32_t pos0, int32_t n,
+                          void *k_out, const mxfa_strides *k_strides, void *v_out, const mxfa_strides *v_strides,
+                          void *stream);
+
+/* Attention of seq_q new queries of every sequence over a 4-bit cache.  Sequence b has kv_len[b] keys
+ * (device int32 [B], clamped to 0 .. seq_k; its own new tokens, appended before, included) and query i
+ * is its position kv_len[b] - seq_q + i: one call for a decode step, drafted tokens to verify, a
+ * prompt chunk or a whole prompt.  With kv_len NULL every sequence has seq_k keys and query i is position
+ * q_pos0 + i.  A query that sees no key (an empty slot of the batch, a position below 0) gives 0. */
+typedef struct {
+  int32_t batch, num_q_heads, num_kv_heads; /* query head h reads KV head h / (Hq/Hkv)                    */
+  int32_t seq_q, seq_k;                     /* seq_k: most keys of any sequence (any number)              */
+  int32_t head_dim;                         /* 64, 128 or 256                                             */
+  int32_t max_len;                          /* the cache's capacity                                       */
+  int32_t causal;                           /* key kpos masked when kpos > the query's position           */
+  int32_t q_pos0;                           /* position of query 0 where kv_len is NULL                   */
+  int32_t window;                           /* 0 = off; else kpos masked when kpos + window <= position    */
+  float   softmax_scale;                    /* normally 1/sqrt(D)                                         */
+  float   softcap;                          /* 0 = off; s <- cap*tanh(s/cap) after scale                  */
+  int32_t o_fmt;                            /* mxfa_c_fmt of O                                            */
+} mxfa_kv4_attn_params;
+
+/* n_parts: parts of the key range that are merged through the workspace (1: none, and workspace_bytes
+ * is 0). */
+mxfa_status mxfa_kv4_attention_plan(const mxfa_kv4_attn_params *p, int32_t *n_parts, size_t *workspace_bytes);
+
+/* q: bf16 rows [B][Hq][seq_q][D] as q_strides say; o: bf16 or fp32 rows as o_strides say.  Scores and sums
+ * are fp32, of the exact cache values; P enters the PV product as two bf16 terms for bf16 O (2^-17 of
+ * P), three for fp32 O (2^-25).  Calls that overlap need a workspace each. */
+mxfa_status mxfa_kv4_attention(const mxfa_kv4_attn_params *p, const void *q, const mxfa_strides *q_strides,
+                               const uint8_t *k_cache, const uint8_t *k_sc, const uint8_t *v_cache,
+                               const uint8_t *v_sc, const int32_t *kv_len, void *o, const mxfa_strides *o_strides,
+                               void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- RMS norm to MX operands ---- */
+
+typedef struct {
+  int64_t rows;
+  int32_t cols;                             /* multiple of 32                                             */
+  int32_t x_fmt;                            /* mxfa_c_fmt of x, residual, weight and h                     */
+  float   eps;                              /* added to the mean square                                   */
+  float   weight_offset;                    /* added to the weight (1 where a model stores w - 1)          */
+  int64_t scale_stride;                     /* 0: scales [rows][cols/32] (mxfa_quantize_rows'); else      */
+                                            /* [cols/32][scale_stride], mxfa_gemm's A scales, >= rows      */
+} mxfa_norm_params;
+
+/* The norm in front of a projection, to the operand that mxfa_gemm takes: h = x + residual, rounded to
+ * x_fmt and written to h (residual NULL: h = x, and h may be NULL), y = h / sqrt(mean(h^2) + eps) * (weight +
+ * weight_offset) in fp32, y to E4M3 codes [rows][cols] and scales by rule R1 (the codes of
+ * mxfa_quantize_rows).  x, residual, h [rows][cols]; h may be x or residual (the same tensor, in place). */
+mxfa_status mxfa_rmsnorm_quantize(const mxfa_norm_params *p, const void *x, const void *residual, const void *weight,
+                                  void *h, uint8_t *codes, uint8_t *scales, void *stream);
+
 /* Synthetic inputs: x[i] ~ N(0,1) (counter-based hash + Box-Muller), each element
  * multiplied by outlier_mul with probability outlier_p.  Replaces make_inputs /
  * make_inputs_gqa (kernels/flash_attention_mx_gqa/flash_attention_model.py:58-65,166-172). */

@@ -1,0 +1,91 @@
+// RMS norm with the residual's addition and MX E4M3 output.
+#pragma once
+
+#include "k_kv4.hip"
+
+// h = x + residual (rounded to their type; without a residual h is x), y = h / sqrt(mean(h^2) + eps) * (w +
+// w_offset) in fp32, y to E4M3 codes and E8M0 scales of rule R1, 32-blocks along the row.  The norm is that
+// of the h that is stored, so whoever reads h sees what was normed.  One workgroup per row; a thread
+// holds 8 consecutive elements (a quarter of a block) of up to NORM_J chunks 2,048 apart in registers between
+// the sum and the output, and reads the chunks of a longer row again.
+constexpr int NORM_J = 4;
+
+template <bool F32>
+__device__ __forceinline__ void norm_store8(void* base, int64_t off, const float (&x)[8]) {
+  if constexpr (F32) {
+    float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + off);
+    p[0] = make_float4(x[0], x[1], x[2], x[3]);
+    p[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    v4i w;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = (int)pack_bf16(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<v4i*>(static_cast<uint16_t*>(base) + off) = w;
+  }
+}
+
+template <bool F32>
+__device__ __forceinline__ void norm_quant_impl(const NormArgs& a) {
+  __shared__ float ssum[4];
+  const int tid = threadIdx.x, nchunk = a.cols / 8;
+  const int64_t row = blockIdx.x, base = row * a.cols;
+  auto load_h = [&](float (&h)[8], int c) {
+    kv4_load8<F32>(h, a.x, base + 8 * c);
+    if (a.residual) {
+      float r[8];
+      kv4_load8<F32>(r, a.residual, base + 8 * c);
+#pragma unroll
+      for (int i = 0; i < 8; i++) h[i] = F32 ? h[i] + r[i] : (float)(__bf16)(h[i] + r[i]);
+    }
+  };
+  float h[NORM_J][8], ss = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NORM_J; j++) {
+    const int c = tid + 256 * j;
+    if (c < nchunk) {
+      load_h(h[j], c);
+#pragma unroll
+      for (int i = 0; i < 8; i++) ss = __builtin_fmaf(h[j][i], h[j][i], ss);
+    }
+  }
+  for (int c = tid + 256 * NORM_J; c < nchunk; c += 256) {
+    float t[8];
+    load_h(t, c);
+#pragma unroll
+    for (int i = 0; i < 8; i++) ss = __builtin_fmaf(t[i], t[i], ss);
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) ss += __shfl_xor(ss, k);
+  if ((tid & 63) == 0) ssum[tid >> 6] = ss;
+  __syncthreads();
+  const float inv = 1.0f / __builtin_sqrtf((ssum[0] + ssum[1] + ssum[2] + ssum[3]) / (float)a.cols + a.eps);
+  auto put = [&](float (&t)[8], int c) {
+    if (a.h) norm_store8<F32>(a.h, base + 8 * c, t);
+    float w[8], m = 0.0f;
+    kv4_load8<F32>(w, a.w, 8 * c);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      t[i] = t[i] * inv * (w[i] + a.w_offset);
+      m = fmaxf(m, fabsf(t[i]));
+    }
+    const uint32_t sc = scale_code(max4(m), 8);
+#pragma unroll
+    for (int i = 0; i < 8; i++) t[i] = __builtin_ldexpf(t[i], 127 - (int)sc);
+    const uint2 codes = make_uint2(e4m3_code4(t[0], t[1], t[2], t[3]), e4m3_code4(t[4], t[5], t[6], t[7]));
+    *reinterpret_cast<uint2*>(a.codes + base + 8 * c) = codes;
+    if ((c & 3) == 0) a.scales[a.sc_ld ? (c >> 2) * a.sc_ld + row : row * (a.cols / 32) + (c >> 2)] = (uint8_t)sc;
+  };
+#pragma unroll
+  for (int j = 0; j < NORM_J; j++) {
+    const int c = tid + 256 * j;
+    if (c < nchunk) put(h[j], c);
+  }
+  for (int c = tid + 256 * NORM_J; c < nchunk; c += 256) {
+    float t[8];
+    load_h(t, c);
+    put(t, c);
+  }
+}
+
+extern "C" __global__ void __launch_bounds__(256) mxfa_rmsnorm_quant_f32(NormArgs a) { norm_quant_impl<true>(a); }
+extern "C" __global__ void __launch_bounds__(256) mxfa_rmsnorm_quant_bf16(NormArgs a) { norm_quant_impl<false>(a); }

@@ -55,3 +55,50 @@ struct GemmArgs {
   int tiles_n;        // number of 256-column tiles
   int c_bf16;         // C is written as bf16 (round to nearest even)
 };
+
+// 4-bit KV cache: append and read-back.  Element strides between batches, heads and tokens of the
+// caller's K and V rows (k_new / v_new, or k_out / v_out).
+struct Kv4CopyArgs {
+  void* kx;
+  void* vx;
+  int64_t k_b, k_h, k_t, v_b, v_h, v_t;
+  uint8_t* k;
+  uint8_t* ks;
+  uint8_t* v;
+  uint8_t* vs;
+  const int* pos;     // first position of each sequence [B], or NULL: pos0
+  const int* counts;  // append: tokens of each sequence that count [B], or NULL: n
+  int pos0, n, B, H, D, L;
+};
+
+// Attention over a 4-bit KV cache (mxfa_kv4_attention).
+struct Kv4AttnArgs {
+  const uint8_t* q;   // bf16
+  const uint8_t* k;
+  const uint8_t* ks;
+  const uint8_t* v;
+  const uint8_t* vs;
+  const int* kv_len;  // keys of each sequence [B], or NULL: Sk
+  uint8_t* o;         // bf16 or fp32
+  float* part_o;      // [B * Hkv * rows][n_parts][D], unnormalized
+  float* part_ml;     // [B * Hkv * rows][n_parts][2]: the reference exponent (log2 units) and the row sum
+  int64_t q_b, q_h, q_t, o_b, o_h, o_t;   // element strides
+  int B, Hq, Hkv, Sq, Sk, L;
+  int group, rows;    // Hq / Hkv; rows of a KV head: group * Sq, row r = query r / group of head r % group
+  int q_pos0, window, causal, o_bf16;
+  int n_rt, n_parts;  // row tiles of a KV head; parts of the key range
+  float c_log2, sc_u, cap_log2;
+};
+
+// RMS norm with the residual's addition and MX E4M3 output (mxfa_rmsnorm_quantize).
+struct NormArgs {
+  const void* x;
+  const void* residual;   // or NULL
+  const void* w;
+  void* h;                // x + residual, or NULL
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t rows, sc_ld;    // sc_ld > 0: scales [cols/32][sc_ld]; 0: [rows][cols/32]
+  int cols;
+  float eps, w_offset;
+};

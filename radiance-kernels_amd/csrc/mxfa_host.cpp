@@ -82,6 +82,11 @@ const char* const kKernelNames[] = {
   "mxfa_decode_d" #D "_blk", "mxfa_decode_d" #D "_softcap_blk", "mxfa_decode_d" #D "_r2_blk", \
       "mxfa_decode_d" #D "_softcap_r2_blk"
     MXFA_DECODE_BLK_NAMES(64), MXFA_DECODE_BLK_NAMES(128), MXFA_DECODE_BLK_NAMES(256),
+    "mxfa_kv4_append_f32", "mxfa_kv4_append_bf16", "mxfa_kv4_read_f32", "mxfa_kv4_read_bf16", "mxfa_kv4_combine",
+    "mxfa_rmsnorm_quant_f32", "mxfa_rmsnorm_quant_bf16",
+#define MXFA_KV4_NAMES(D) \
+  "mxfa_kv4_attn_d" #D, "mxfa_kv4_attn_d" #D "_softcap", "mxfa_kv4_attn_d" #D "_f32", "mxfa_kv4_attn_d" #D "_softcap_f32"
+    MXFA_KV4_NAMES(64), MXFA_KV4_NAMES(128), MXFA_KV4_NAMES(256),
 };
 constexpr int kNumKernels = sizeof(kKernelNames) / sizeof(kKernelNames[0]);
 
@@ -926,6 +931,226 @@ mxfa_status mxfa_decode_noalloc(const mxfa_attn_params* p, const uint8_t* q, con
   DeviceModule* dm;
   if (mxfa_status st = loaded_module_for_current(&dm)) return st;
   return decode_launch(dm, p, q, q_sc, k_cache, k_sc, v_cache, v_sc, o, dm->decode_scratch, stream);
+}
+
+}  // extern "C"
+
+// ---- 4-bit KV cache -----------------------------------------------------------------------
+
+namespace {
+
+mxfa_status check_kv4_shape(const mxfa_kv4_shape* c) {
+  if (!c) return fail(MXFA_ERR_INVALID_ARG, "the cache's shape is NULL");
+  if (c->batch < 1 || c->num_kv_heads < 1) return fail(MXFA_ERR_INVALID_ARG, "batch and num_kv_heads must be >= 1");
+  if (c->head_dim < 32 || c->head_dim % 32) return fail(MXFA_ERR_INVALID_ARG, "head_dim must be a positive multiple of 32");
+  if (c->max_len < 32 || c->max_len % 32) return fail(MXFA_ERR_INVALID_ARG, "max_len must be a positive multiple of 32");
+  return MXFA_OK;
+}
+
+// Strides of rows of `dim` elements, for `rows` of them in a head (all 0: dense [batch][head][rows][dim]), which
+// keep every row at a multiple of `align` elements.
+mxfa_status resolve_strides(const mxfa_strides* st, int64_t heads, int64_t rows, int64_t dim, int align, const char* what,
+                            int64_t* b, int64_t* h, int64_t* t) {
+  if (!st || (st->batch == 0 && st->head == 0 && st->token == 0)) {
+    *t = dim;
+    *h = rows * dim;
+    *b = heads * rows * dim;
+    return MXFA_OK;
+  }
+  if (st->batch % align || st->head % align || st->token % align)
+    return fail(MXFA_ERR_INVALID_ARG, std::string(what) + " strides must be multiples of " + std::to_string(align) + " elements");
+  *b = st->batch;
+  *h = st->head;
+  *t = st->token;
+  return MXFA_OK;
+}
+
+mxfa_status kv4_copy(const char* kind, const mxfa_kv4_shape* c, int32_t x_fmt, const void* kx, const mxfa_strides* k_st,
+                     const void* vx, const mxfa_strides* v_st, const int32_t* pos, int32_t pos0, const int32_t* counts, int32_t n,
+                     const uint8_t* k, const uint8_t* k_sc, const uint8_t* v, const uint8_t* v_sc, void* stream) {
+  if (mxfa_status st = check_kv4_shape(c)) return st;
+  if (x_fmt != MXFA_C_F32 && x_fmt != MXFA_C_BF16) return fail(MXFA_ERR_INVALID_ARG, "x_fmt must be MXFA_C_F32 or MXFA_C_BF16");
+  if (n < 0) return fail(MXFA_ERR_INVALID_ARG, "the number of tokens must be >= 0");
+  if (!pos && (pos0 < 0 || (int64_t)pos0 + n > c->max_len))
+    return fail(MXFA_ERR_INVALID_ARG, "need 0 <= pos0 and pos0 + the number of tokens <= max_len");
+  if (n == 0) return MXFA_OK;
+  const void* ptrs[] = {kx, vx, k, k_sc, v, v_sc};
+  if (mxfa_status st = check_ptrs(ptrs, 6)) return st;
+  for (const int32_t* q : {pos, counts})
+    if (reinterpret_cast<uintptr_t>(q) & 3u) return fail(MXFA_ERR_INVALID_ARG, "pos and counts must be 4-byte aligned");
+  Kv4CopyArgs a;
+  std::memset(&a, 0, sizeof a);
+  const int align = x_fmt == MXFA_C_F32 ? 4 : 8;
+  if (mxfa_status st = resolve_strides(k_st, c->num_kv_heads, n, c->head_dim, align, "K", &a.k_b, &a.k_h, &a.k_t)) return st;
+  if (mxfa_status st = resolve_strides(v_st, c->num_kv_heads, n, c->head_dim, align, "V", &a.v_b, &a.v_h, &a.v_t)) return st;
+  a.kx = const_cast<void*>(kx); a.vx = const_cast<void*>(vx);
+  a.k = const_cast<uint8_t*>(k); a.ks = const_cast<uint8_t*>(k_sc);
+  a.v = const_cast<uint8_t*>(v); a.vs = const_cast<uint8_t*>(v_sc);
+  a.pos = pos; a.counts = counts; a.pos0 = pos0; a.n = n;
+  a.B = c->batch; a.H = c->num_kv_heads; a.D = c->head_dim; a.L = c->max_len;
+  // (each factor below 2^31, so the first product cannot overflow; the second is checked against 2^32)
+  const int64_t bh = (int64_t)c->batch * c->num_kv_heads, units = (int64_t)n * (c->head_dim / 8);
+  if (bh > (int64_t)UINT32_MAX / units) return fail(MXFA_ERR_UNSUPPORTED, "the call needs more than 2^32 work-items in one launch: split it");
+  const int64_t blocks = (bh * units + 255) / 256;
+  if (mxfa_status st = check_grid(blocks, 256)) return st;
+  DeviceModule* dm;
+  if (mxfa_status st = module_for_current(&dm)) return st;
+  char name[40];
+  std::snprintf(name, sizeof name, "mxfa_kv4_%s_%s", kind, x_fmt == MXFA_C_F32 ? "f32" : "bf16");
+  void* args[] = {&a};
+  return launch(dm, name, dim3((unsigned)blocks), dim3(256), args, stream);
+}
+
+mxfa_status check_kv4_attn(const mxfa_kv4_attn_params* p) {
+  if (!p) return fail(MXFA_ERR_INVALID_ARG, "params is NULL");
+  if (p->batch < 1 || p->num_q_heads < 1 || p->num_kv_heads < 1 || p->seq_q < 1 || p->seq_k < 1)
+    return fail(MXFA_ERR_INVALID_ARG, "batch, heads, seq_q and seq_k must be >= 1");
+  if (p->num_q_heads % p->num_kv_heads) return fail(MXFA_ERR_INVALID_ARG, "num_q_heads must be a multiple of num_kv_heads");
+  if (p->head_dim < 32 || p->head_dim % 32) return fail(MXFA_ERR_INVALID_ARG, "head_dim must be a positive multiple of 32");
+  if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+    return fail(MXFA_ERR_UNSUPPORTED, "head_dim must be 64, 128 or 256");
+  if (p->max_len < 32 || p->max_len % 32 || p->max_len < p->seq_k)
+    return fail(MXFA_ERR_INVALID_ARG, "max_len must be a multiple of 32 that is >= seq_k");
+  if (p->q_pos0 < 0 || p->window < 0) return fail(MXFA_ERR_INVALID_ARG, "q_pos0 and window must be >= 0");
+  if (!(p->softmax_scale > 0.0f) || !std::isfinite(p->softmax_scale))
+    return fail(MXFA_ERR_INVALID_ARG, "softmax_scale must be finite and > 0");
+  if (!(p->softcap >= 0.0f) || !std::isfinite(p->softcap)) return fail(MXFA_ERR_INVALID_ARG, "softcap must be finite and >= 0");
+  if (p->o_fmt != MXFA_C_F32 && p->o_fmt != MXFA_C_BF16) return fail(MXFA_ERR_INVALID_ARG, "o_fmt must be MXFA_C_F32 or MXFA_C_BF16");
+  // a (batch, KV head)'s codes are addressed with 32-bit byte offsets, positions with 32-bit sums
+  if ((int64_t)p->max_len * (p->head_dim / 2) > (int64_t)INT32_MAX)
+    return fail(MXFA_ERR_UNSUPPORTED, "max_len * head_dim exceeds the kernels' 32-bit K/V range (2^32 elements per head)");
+  if ((int64_t)p->q_pos0 + p->seq_q > ((int64_t)1 << 30)) return fail(MXFA_ERR_UNSUPPORTED, "q_pos0 + seq_q must be at most 2^30");
+  if ((int64_t)(p->num_q_heads / p->num_kv_heads) * p->seq_q > ((int64_t)1 << 30))
+    return fail(MXFA_ERR_UNSUPPORTED, "at most 2^30 query rows per KV head");
+  return MXFA_OK;
+}
+
+// How a call is dealt to workgroups.
+struct Kv4Plan {
+  int n_rt, n_parts;       // row tiles of a KV head; parts of the key range
+  int64_t items;           // workgroups
+  size_t ws;
+};
+
+mxfa_status kv4_plan(const mxfa_kv4_attn_params* p, Kv4Plan* out) {
+  const int64_t rows = (int64_t)(p->num_q_heads / p->num_kv_heads) * p->seq_q;
+  const int64_t bk = (int64_t)p->batch * p->num_kv_heads;
+  out->n_rt = (int)((rows + 15) / 16);
+  if (bk > (int64_t)UINT32_MAX / 256 / out->n_rt)
+    return fail(MXFA_ERR_UNSUPPORTED, "the call needs more than 2^32 work-items in one launch: split it");
+  const int64_t tiles = bk * out->n_rt, blocks = (p->seq_k + 63) / 64;
+  int64_t n = std::min<int64_t>((512 + tiles - 1) / tiles, (blocks + 3) / 4);
+  out->n_parts = (int)std::max<int64_t>(n, 1);
+  out->items = tiles * out->n_parts;
+  out->ws = out->n_parts > 1 ? (size_t)bk * rows * out->n_parts * (p->head_dim + 2) * sizeof(float) : 0;
+  return MXFA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+mxfa_status mxfa_kv4_append(const mxfa_kv4_shape* c, int32_t x_fmt, const void* k_new, const mxfa_strides* k_strides,
+                            const void* v_new, const mxfa_strides* v_strides, const int32_t* pos, int32_t pos0,
+                            const int32_t* counts, int32_t n_new, uint8_t* k_cache, uint8_t* k_sc, uint8_t* v_cache,
+                            uint8_t* v_sc, void* stream) {
+  return kv4_copy("append", c, x_fmt, k_new, k_strides, v_new, v_strides, pos, pos0, counts, n_new, k_cache, k_sc, v_cache,
+                  v_sc, stream);
+}
+
+mxfa_status mxfa_kv4_read(const mxfa_kv4_shape* c, int32_t x_fmt, const uint8_t* k_cache, const uint8_t* k_sc,
+                          const uint8_t* v_cache, const uint8_t* v_sc, const int32_t* pos, int32_t pos0, int32_t n, void* k_out,
+                          const mxfa_strides* k_strides, void* v_out, const mxfa_strides* v_strides, void* stream) {
+  return kv4_copy("read", c, x_fmt, k_out, k_strides, v_out, v_strides, pos, pos0, nullptr, n, k_cache, k_sc, v_cache, v_sc,
+                  stream);
+}
+
+mxfa_status mxfa_kv4_attention_plan(const mxfa_kv4_attn_params* p, int32_t* n_parts, size_t* workspace_bytes) {
+  if (mxfa_status st = check_kv4_attn(p)) return st;
+  Kv4Plan plan;
+  if (mxfa_status st = kv4_plan(p, &plan)) return st;
+  if (n_parts) *n_parts = plan.n_parts;
+  if (workspace_bytes) *workspace_bytes = plan.ws;
+  return MXFA_OK;
+}
+
+mxfa_status mxfa_kv4_attention(const mxfa_kv4_attn_params* p, const void* q, const mxfa_strides* q_strides,
+                               const uint8_t* k_cache, const uint8_t* k_sc, const uint8_t* v_cache, const uint8_t* v_sc,
+                               const int32_t* kv_len, void* o, const mxfa_strides* o_strides, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  if (mxfa_status st = check_kv4_attn(p)) return st;
+  const void* ptrs[] = {q, k_cache, k_sc, v_cache, v_sc, o};
+  if (mxfa_status st = check_ptrs(ptrs, 6)) return st;
+  if (reinterpret_cast<uintptr_t>(kv_len) & 3u) return fail(MXFA_ERR_INVALID_ARG, "kv_len must be 4-byte aligned");
+  Kv4AttnArgs a;
+  std::memset(&a, 0, sizeof a);
+  const bool bf16 = p->o_fmt == MXFA_C_BF16;
+  if (mxfa_status st = resolve_strides(q_strides, p->num_q_heads, p->seq_q, p->head_dim, 8, "q", &a.q_b, &a.q_h, &a.q_t)) return st;
+  if (mxfa_status st = resolve_strides(o_strides, p->num_q_heads, p->seq_q, p->head_dim, bf16 ? 8 : 4, "o", &a.o_b, &a.o_h, &a.o_t))
+    return st;
+  Kv4Plan plan;
+  if (mxfa_status st = kv4_plan(p, &plan)) return st;
+  if (plan.ws && (!workspace || workspace_bytes < plan.ws))
+    return fail(MXFA_ERR_WORKSPACE, "attention workspace needs " + std::to_string(plan.ws) + " bytes");
+  if (!aligned16(workspace)) return fail(MXFA_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+  a.q = static_cast<const uint8_t*>(q); a.k = k_cache; a.ks = k_sc; a.v = v_cache; a.vs = v_sc;
+  a.kv_len = kv_len; a.o = static_cast<uint8_t*>(o);
+  a.B = p->batch; a.Hq = p->num_q_heads; a.Hkv = p->num_kv_heads; a.Sq = p->seq_q; a.Sk = p->seq_k; a.L = p->max_len;
+  a.group = p->num_q_heads / p->num_kv_heads;
+  a.rows = a.group * p->seq_q;
+  a.q_pos0 = p->q_pos0;
+  a.window = p->window < (1 << 30) ? p->window : 0;              // (positions stay below 2^30: no key is that far behind)
+  a.causal = p->causal != 0;
+  a.o_bf16 = bf16;
+  a.n_rt = plan.n_rt; a.n_parts = plan.n_parts;
+  const float log2e = 1.4426950408889634f;
+  a.c_log2 = p->softmax_scale * log2e;
+  if (p->softcap > 0.0f) {
+    a.sc_u = p->softmax_scale / p->softcap;
+    a.cap_log2 = p->softcap * log2e;
+  }
+  const int64_t rows = (int64_t)p->batch * p->num_kv_heads * a.rows;
+  if (plan.n_parts > 1) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + rows * plan.n_parts * p->head_dim;
+  }
+  if (mxfa_status st = check_grid(plan.items, 256)) return st;
+  if (mxfa_status st = check_grid(plan.n_parts > 1 ? rows : 0, p->head_dim)) return st;
+  DeviceModule* dm;
+  if (mxfa_status st = module_for_current(&dm)) return st;
+  char name[48];
+  std::snprintf(name, sizeof name, "mxfa_kv4_attn_d%d%s%s", p->head_dim, p->softcap > 0.0f ? "_softcap" : "", bf16 ? "" : "_f32");
+  void* args[] = {&a};
+  if (mxfa_status st = launch(dm, name, dim3((unsigned)plan.items), dim3(256), args, stream)) return st;
+  if (plan.n_parts == 1) return MXFA_OK;
+  return launch(dm, "mxfa_kv4_combine", dim3((unsigned)rows), dim3((unsigned)p->head_dim), args, stream);
+}
+
+mxfa_status mxfa_rmsnorm_quantize(const mxfa_norm_params* p, const void* x, const void* residual, const void* weight, void* h,
+                                  uint8_t* codes, uint8_t* scales, void* stream) {
+  if (!p) return fail(MXFA_ERR_INVALID_ARG, "params is NULL");
+  if (p->rows < 0 || p->cols < 32 || p->cols % 32) return fail(MXFA_ERR_INVALID_ARG, "cols must be a positive multiple of 32 and rows >= 0");
+  if (p->x_fmt != MXFA_C_F32 && p->x_fmt != MXFA_C_BF16) return fail(MXFA_ERR_INVALID_ARG, "x_fmt must be MXFA_C_F32 or MXFA_C_BF16");
+  if (!(p->eps >= 0.0f) || !std::isfinite(p->eps) || !std::isfinite(p->weight_offset))
+    return fail(MXFA_ERR_INVALID_ARG, "eps must be finite and >= 0, weight_offset finite");
+  if (p->scale_stride != 0 && p->scale_stride < p->rows)
+    return fail(MXFA_ERR_INVALID_ARG, "scale_stride must be 0 or at least rows");
+  if (p->rows == 0) return MXFA_OK;
+  const void* ptrs[] = {x, weight, codes};
+  if (mxfa_status st = check_ptrs(ptrs, 3)) return st;
+  if (!scales) return fail(MXFA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (!aligned16(residual) || !aligned16(h)) return fail(MXFA_ERR_INVALID_ARG, "tensor pointers must be 16-byte aligned");
+  if (residual && !h) return fail(MXFA_ERR_INVALID_ARG, "a residual needs h");
+  if (mxfa_status st = check_grid(p->rows, 256)) return st;
+  NormArgs a;
+  std::memset(&a, 0, sizeof a);
+  a.x = x; a.residual = residual; a.w = weight; a.h = h; a.codes = codes; a.scales = scales;
+  a.rows = p->rows; a.sc_ld = p->scale_stride; a.cols = p->cols; a.eps = p->eps; a.w_offset = p->weight_offset;
+  DeviceModule* dm;
+  if (mxfa_status st = module_for_current(&dm)) return st;
+  void* args[] = {&a};
+  return launch(dm, p->x_fmt == MXFA_C_F32 ? "mxfa_rmsnorm_quant_f32" : "mxfa_rmsnorm_quant_bf16", dim3((unsigned)p->rows), dim3(256),
+                args, stream);
 }
 
 }  // extern "C"

@@ -9,6 +9,8 @@
 //   k_prefill.hip      bf16-K pre-pass, prefill (workspace, workspace-free, stage trace)
 //   k_decode.hip       split-KV decode, partials merge
 //   k_gemm.hip         MX GEMM (register-staged, LDS-DMA, skinny)
+//   k_kv4.hip          4-bit KV cache: append, read-back, attention
+//   k_norm.hip         RMS norm with the residual's addition and MX E4M3 output
 //
 // Reference path (ucb-bar/radiance-kernels): kernels/flash_attention_mx{,_gqa,
 // _gemma,_fp6,_stable}.  Per key block the reference runs QK^T on the MX mesh,
@@ -46,3 +48,5 @@
 #include "k_prefill.hip"
 #include "k_decode.hip"
 #include "k_gemm.hip"
+#include "k_kv4.hip"
+#include "k_norm.hip"

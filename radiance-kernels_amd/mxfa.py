@@ -14,6 +14,8 @@ vocabulary on top of the C ABI:
     decode            -> the same recurrence over an MXFP8 KV cache (split-KV)
     softmax_requant   -> fused_softmax_requant (the P tile step, for bit-exact checks)
     KvCache.append    -> the producer side of decode: new tokens into the MXFP8 cache
+    Kv4Cache, kv4_attention -> a cache held in 4 bits (E2M1, per token) and attention over it
+    rmsnorm_quantize  -> residual addition, RMS norm and MX codes in front of a projection
 
 torch is used only to hold device memory and name the stream; every call goes through
 ctypes into libmxfa.so, which launches gfx950 kernels.  There is no fallback: if the
@@ -104,10 +106,34 @@ class GemmParams(ctypes.Structure):
                 ("a_fmt", ctypes.c_int32), ("b_fmt", ctypes.c_int32), ("c_fmt", ctypes.c_int32)]
 
 
+class Kv4Shape(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("max_len", ctypes.c_int32)]
+
+
+class Strides(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("head", ctypes.c_int64), ("token", ctypes.c_int64)]
+
+
+class Kv4AttnParams(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("num_q_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("seq_q", ctypes.c_int32), ("seq_k", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("max_len", ctypes.c_int32), ("causal", ctypes.c_int32), ("q_pos0", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("o_fmt", ctypes.c_int32),
+    ]
+
+
+class NormParams(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_int64), ("cols", ctypes.c_int32), ("x_fmt", ctypes.c_int32), ("eps", ctypes.c_float),
+                ("weight_offset", ctypes.c_float), ("scale_stride", ctypes.c_int64)]
+
+
 EXPORTS = ("mxfa_quantize_rows", "mxfa_quantize_rows_r4", "mxfa_quantize_cols", "mxfa_prefill", "mxfa_prefill_plan",
            "mxfa_prefill_ws", "mxfa_prefill_trace", "mxfa_decode_plan", "mxfa_decode", "mxfa_decode_noalloc",
            "mxfa_kv_append", "mxfa_softmax_requant", "mxfa_fill_normal", "mxfa_init", "mxfa_shutdown", "mxfa_status_string",
-           "mxfa_last_error", "mxfa_version", "mxfa_gemm")
+           "mxfa_last_error", "mxfa_version", "mxfa_gemm", "mxfa_kv4_append", "mxfa_kv4_read", "mxfa_kv4_attention_plan",
+           "mxfa_kv4_attention", "mxfa_rmsnorm_quantize")
 
 _lib = None
 
@@ -137,13 +163,21 @@ def lib():
         L.mxfa_fill_normal.argtypes = [f32p, ctypes.c_int64, ctypes.c_uint64, ctypes.c_float, ctypes.c_float, vp]
         L.mxfa_kv_append.argtypes = [P(KvParams), f32p, f32p, ctypes.c_int32, ctypes.c_int32] + [u8p] * 4 + [f32p, vp]
         L.mxfa_gemm.argtypes = [P(GemmParams), u8p, u8p, u8p, u8p, vp, vp]
+        i32, st = ctypes.c_int32, P(Strides)
+        L.mxfa_kv4_append.argtypes = [P(Kv4Shape), i32, vp, st, vp, st, vp, i32, vp, i32] + [u8p] * 4 + [vp]
+        L.mxfa_kv4_read.argtypes = [P(Kv4Shape), i32] + [u8p] * 4 + [vp, i32, i32, vp, st, vp, st, vp]
+        L.mxfa_kv4_attention_plan.argtypes = [P(Kv4AttnParams), P(i32), P(ctypes.c_size_t)]
+        L.mxfa_kv4_attention.argtypes = [P(Kv4AttnParams), vp, st] + [u8p] * 4 + [vp, vp, st, vp, ctypes.c_size_t, vp]
+        L.mxfa_rmsnorm_quantize.argtypes = [P(NormParams), vp, vp, vp, vp, u8p, u8p, vp]
         L.mxfa_status_string.argtypes = [ctypes.c_int]
         L.mxfa_status_string.restype = ctypes.c_char_p
         L.mxfa_last_error.restype = ctypes.c_char_p
         L.mxfa_version.restype = ctypes.c_int32
         for name in ("mxfa_quantize_rows", "mxfa_quantize_rows_r4", "mxfa_quantize_cols", "mxfa_prefill",
                      "mxfa_prefill_plan", "mxfa_prefill_ws", "mxfa_prefill_trace", "mxfa_decode_plan", "mxfa_decode",
-                     "mxfa_decode_noalloc", "mxfa_softmax_requant", "mxfa_fill_normal", "mxfa_init", "mxfa_kv_append", "mxfa_gemm"):
+                     "mxfa_decode_noalloc", "mxfa_softmax_requant", "mxfa_fill_normal", "mxfa_init", "mxfa_kv_append", "mxfa_gemm",
+                     "mxfa_kv4_append", "mxfa_kv4_read", "mxfa_kv4_attention_plan", "mxfa_kv4_attention",
+                     "mxfa_rmsnorm_quantize"):
             getattr(L, name).restype = ctypes.c_int
         _lib = L
     return _lib
@@ -427,6 +461,195 @@ class KvCache:
                                     _ptr(self.k), _ptr(self.ks), _ptr(self.v), _ptr(self.vs), _ptr(self.tail),
                                     _stream(stream)))
         self.length += n
+
+
+# ---- 4-bit KV cache (mxfa_kv4_*) and the norm in front of a projection -------------------------
+
+def _x_fmt(t, name):
+    import torch
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise MxfaError(1, f"{name} must be a CUDA tensor")
+    if t.dtype is torch.bfloat16:
+        return C_BF16
+    if t.dtype is torch.float32:
+        return C_F32
+    raise MxfaError(1, f"{name} must be float32 or bfloat16, got {t.dtype}")
+
+
+def _rows(t, dtype, shape, device, name, written=False):
+    """mxfa_strides of a [B, H, n, D] tensor whose rows of D are contiguous (None: dense), after a check of its
+    device, dtype and shape.  written: rows must not share memory."""
+    import torch
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device == device):
+        raise MxfaError(1, f"{name} must be a tensor on {device}")
+    if t.dtype is not dtype:
+        raise MxfaError(1, f"{name} must be {dtype}, got {t.dtype}")
+    if t.shape != shape:
+        raise MxfaError(1, f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.is_contiguous():
+        return None
+    b, h, n, d = t.stride()
+    if d != 1:
+        raise MxfaError(1, f"{name}: the elements of a row must be contiguous")
+    # (an axis of one element may have any stride)
+    used = [(s, m) for s, m in zip((b, h, n), shape) if m > 1]
+    if not used:
+        return None
+    if all(s == 0 for s, _ in used) or (written and any(s == 0 for s, _ in used)):
+        raise MxfaError(1, f"{name} is broadcast")
+    return Strides(b if shape[0] > 1 else 0, h if shape[1] > 1 else 0, n if shape[2] > 1 else 0)
+
+
+def _index(t, n, device, name):
+    """Pointer of an int32 [n] tensor on `device`, or None."""
+    import torch
+    if t is None:
+        return None
+    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()):
+        raise MxfaError(1, f"{name} must be a contiguous int32 tensor of shape ({n},) on {device}")
+    return t.data_ptr()
+
+
+def _on(device):
+    """The library launches on the current device: a call whose tensors lie elsewhere is refused."""
+    import torch
+    if device.index != torch.cuda.current_device():
+        raise MxfaError(1, f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+class Kv4Cache:
+    """A 4-bit KV cache on the device (layouts in mxfa.h).  Sequences may have lengths of their own: `pos` of
+    append and read and kv_len of kv4_attention are then int32 CUDA tensors [batch], which the caller
+    advances; without them append writes at `length`, the same for every sequence, and advances it."""
+
+    def __init__(self, batch, num_kv_heads, head_dim, max_len, device="cuda:0"):
+        import torch
+        B, H, D, L = batch, num_kv_heads, head_dim, max_len
+        self.shape = Kv4Shape(B, H, D, L)
+        self.k = torch.zeros((B, H, L, D // 2), dtype=torch.uint8, device=device)
+        self.ks = torch.zeros((B, H, L // 32, 4, D // 32, 8), dtype=torch.uint8, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.vs = torch.zeros_like(self.ks)
+        self.length = 0
+
+    @classmethod
+    def of(cls, k, ks, v, vs, length=0):
+        """A cache in tensors that exist: k, v [B, H, L, D/2] and ks, vs [B, H, L/32, 4, D/32, 8], uint8."""
+        import torch
+        self = cls.__new__(cls)
+        B, H, L, half = k.shape
+        for t, shape, name in ((k, (B, H, L, half), "k"), (ks, (B, H, L // 32, 4, half // 16, 8), "k_sc"),
+                               (v, (B, H, L, half), "v"), (vs, (B, H, L // 32, 4, half // 16, 8), "v_sc")):
+            _need(t, torch.uint8, shape, name)
+            if t.device != k.device:
+                raise MxfaError(1, f"{name} must be on {k.device}")
+        self.shape = Kv4Shape(B, H, 2 * half, L)
+        self.k, self.ks, self.v, self.vs, self.length = k, ks, v, vs, length
+        return self
+
+    def append(self, k_new, v_new, pos=None, counts=None, stream=None):
+        """k_new, v_new: float32 or bfloat16 [B, Hkv, n, D], rows contiguous, the other strides free.  counts:
+        int32 CUDA tensor [B], of each sequence only the first counts[b] tokens are written."""
+        c, dev = self.shape, self.k.device
+        fmt = _x_fmt(k_new, "k_new")
+        shape = (c.batch, c.num_kv_heads, k_new.shape[2] if k_new.dim() == 4 else -1, c.head_dim)
+        ks, vs = _rows(k_new, k_new.dtype, shape, dev, "k_new"), _rows(v_new, k_new.dtype, shape, dev, "v_new")
+        _on(dev)
+        pp, cp = _index(pos, c.batch, dev, "pos"), _index(counts, c.batch, dev, "counts")
+        if pos is None and self.length + shape[2] > c.max_len:
+            raise MxfaError(1, f"append of {shape[2]} tokens at {self.length} exceeds max_len {c.max_len}")
+        _check(lib().mxfa_kv4_append(c, fmt, k_new.data_ptr(), ks, v_new.data_ptr(), vs, pp, self.length if pos is None else 0,
+                                     cp, shape[2], self.k.data_ptr(), self.ks.data_ptr(), self.v.data_ptr(),
+                                     self.vs.data_ptr(), _stream(stream)))
+        if pos is None:
+            self.length += shape[2]
+
+    def read(self, n, pos=0, dtype=None, out=None, stream=None):
+        """(K, V) [B, Hkv, n, D], bfloat16 (default) or float32: the values of n tokens from `pos` (an int, or an
+        int32 CUDA tensor [B]) on.  out: a pair of tensors to write, rows contiguous, the other strides free."""
+        import torch
+        c, dev = self.shape, self.k.device
+        shape = (c.batch, c.num_kv_heads, n, c.head_dim)
+        if out is None:
+            out = tuple(torch.empty(shape, dtype=dtype or torch.bfloat16, device=dev) for _ in range(2))
+        K, V = out
+        fmt = _x_fmt(K, "out[0]")
+        if dtype is not None and K.dtype is not dtype:
+            raise MxfaError(1, f"out[0] must be {dtype}, got {K.dtype}")
+        ks, vs = _rows(K, K.dtype, shape, dev, "out[0]", True), _rows(V, K.dtype, shape, dev, "out[1]", True)
+        _on(dev)
+        ragged = isinstance(pos, torch.Tensor)
+        _check(lib().mxfa_kv4_read(c, fmt, self.k.data_ptr(), self.ks.data_ptr(), self.v.data_ptr(), self.vs.data_ptr(),
+                                   _index(pos, c.batch, dev, "pos") if ragged else None, 0 if ragged else pos, n,
+                                   K.data_ptr(), ks, V.data_ptr(), vs, _stream(stream)))
+        return K, V
+
+
+def make_kv4_params(B, Hq, Hkv, Sq, Sk, D, max_len, causal=True, q_pos0=0, window=0, scale=None, softcap=0.0, o_fmt=C_BF16):
+    return Kv4AttnParams(B, Hq, Hkv, Sq, Sk, D, int(max_len), int(bool(causal)), int(q_pos0), int(window),
+                         float(scale if scale is not None else 1.0 / math.sqrt(D)), float(softcap), int(o_fmt))
+
+
+def kv4_attention_plan(p):
+    """(parts of the key range, workspace bytes) of kv4_attention for p; without parts the bytes are 0."""
+    n, ws = ctypes.c_int32(0), ctypes.c_size_t(0)
+    _check(lib().mxfa_kv4_attention_plan(p, ctypes.byref(n), ctypes.byref(ws)))
+    return n.value, ws.value
+
+
+def kv4_attention(p, q, cache, kv_len=None, out=None, workspace=None, stream=None):
+    """O of new queries over a Kv4Cache (mxfa_kv4_attention): q bfloat16 [B, Hq, Sq, D] and out [B, Hq, Sq, D] of
+    p.o_fmt, rows contiguous, the other strides free; kv_len: int32 CUDA tensor [B], each sequence's keys
+    (None: p.seq_k, queries from p.q_pos0 on).  workspace: a uint8 tensor of kv4_attention_plan's bytes."""
+    import torch
+    c, dev = cache.shape, cache.k.device
+    if (p.batch, p.num_kv_heads, p.head_dim, p.max_len) != (c.batch, c.num_kv_heads, c.head_dim, c.max_len):
+        raise MxfaError(1, "the parameters' batch, num_kv_heads, head_dim and max_len are not the cache's")
+    shape = (p.batch, p.num_q_heads, p.seq_q, p.head_dim)
+    dtype = torch.bfloat16 if p.o_fmt == C_BF16 else torch.float32
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+    qs, os_ = _rows(q, torch.bfloat16, shape, dev, "q"), _rows(out, dtype, shape, dev, "out", True)
+    _on(dev)
+    if workspace is None:
+        workspace = torch.empty(kv4_attention_plan(p)[1], dtype=torch.uint8, device=dev)
+    _need(workspace, torch.uint8, (workspace.numel(),), "workspace")
+    _check(lib().mxfa_kv4_attention(p, q.data_ptr(), qs, cache.k.data_ptr(), cache.ks.data_ptr(), cache.v.data_ptr(),
+                                    cache.vs.data_ptr(), _index(kv_len, p.batch, dev, "kv_len"), out.data_ptr(), os_,
+                                    workspace.data_ptr(), workspace.numel(), _stream(stream)))
+    return out
+
+
+def rmsnorm_quantize(x, weight, eps=1e-6, residual=None, weight_offset=0.0, gemm_scales=False, h=None, stream=None):
+    """(codes, scales, h) of mxfa_rmsnorm_quantize: x [..., cols] float32 or bfloat16, contiguous; residual like x or
+    None (h is then x itself); h: where x + residual goes (residual or x for in place; None allocates).
+    gemm_scales: scales [cols/32, rows], gemm's A scales, else [..., cols/32]."""
+    import torch
+    fmt = _x_fmt(x, "x")
+    cols = x.shape[-1] if x.dim() else 0
+    if cols < 32 or cols % 32:
+        raise MxfaError(1, "cols must be a positive multiple of 32")
+    rows = x.numel() // cols
+    _need(x, x.dtype, x.shape, "x")
+    _need(weight, x.dtype, (cols,), "weight")
+    if residual is None:
+        if h is not None and h is not x:
+            _need(h, x.dtype, x.shape, "h")
+    else:
+        _need(residual, x.dtype, x.shape, "residual")
+        if h is None:
+            h = torch.empty_like(x)
+        _need(h, x.dtype, x.shape, "h")
+    for t, name in ((weight, "weight"), (residual, "residual"), (h, "h")):
+        if t is not None and t.device != x.device:
+            raise MxfaError(1, f"{name} must be on {x.device}")
+    _on(x.device)
+    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
+    scales = torch.empty((cols // 32, rows) if gemm_scales else (*x.shape[:-1], cols // 32), dtype=torch.uint8, device=x.device)
+    p = NormParams(rows, cols, fmt, float(eps), float(weight_offset), rows if gemm_scales else 0)
+    _check(lib().mxfa_rmsnorm_quantize(p, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(h),
+                                       codes.data_ptr(), scales.data_ptr(), _stream(stream)))
+    return codes, scales, x if h is None else h
 
 
 def attention_flops(p):
