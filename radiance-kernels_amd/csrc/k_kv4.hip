@@ -142,9 +142,9 @@ extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_read_f32(Kv4CopyArgs 
 extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_read_bf16(Kv4CopyArgs a) { kv4_read_impl<false>(a); }
 
 // ---------------------------------------------------------------------------
-// Attention, streaming form.  The query rows of a KV head (row r: query r / group of head r %
-// group) are taken 16 at a time as the columns of S^T = K Q^T and O^T += V^T P^T on the 16x16x32 bf16
-// MFMA; K and V are widened to bf16 (exact) in registers, never through LDS.  Lane (n, g) = (lane %
+// Attention, streaming form: at most 32 query rows of a KV head (row r: query r / group of head r %
+// group), NT tiles of 16 of them as the columns of S^T = K Q^T and O^T += V^T P^T on the 16x16x32 bf16
+// MFMA.  K and V are widened to bf16 (exact) in registers, never through LDS.  Lane (n, g) = (lane %
 // 16, lane / 16):
 //   A operand: row n, k = 8 g + e (e < 8); B: column n, k likewise; C: column n, rows 4 g + i (i < 4).
 // Row 4 g + i of a 16-key score tile t of a 32-key group is key 16 t + 4 i + g, so a lane's 8 scores of a
@@ -156,6 +156,12 @@ extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_read_bf16(Kv4CopyArgs
 // The softmax keeps a reference exponent `mc` for each column instead of the running maximum: it is
 // raised (with O and l rescaled) only when a score exceeds it by more than kSlack binades, so P stays
 // below 2^kSlack and a block's maximum crosses lanes only then.
+//
+// Work is dealt in 64-key blocks.  The blocks of all (sequence, KV head) items, laid end to end (as
+// many per sequence as its queries see, at least one), are cut into equal shares, one to a workgroup: no
+// length of a ragged batch leaves a CU idle.  A workgroup walks the pieces of items in its share; a piece
+// that is a whole item is written out, others go to the workspace (slot 2 w for the piece that workgroup
+// w's share begins with, 2 w + 1 for a later one, its last) and mxfa_kv4_combine merges them.
 // ---------------------------------------------------------------------------
 constexpr float kSlack = 4.0f;
 constexpr int KV4_NW = 4;            // waves of a workgroup, each its own key blocks
@@ -180,11 +186,9 @@ __device__ __forceinline__ float scale_byte(uint32_t w, int i) {
   return __uint_as_float(i == 0 ? w << 23 : i == 1 ? w << 15 : i == 2 ? w << 7 : w >> 1);
 }
 
+// Two floats to bf16, nearest even (a in the low half).
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-  v2bf t;
-  t[0] = (__bf16)a;
-  t[1] = (__bf16)b;
-  return __builtin_bit_cast(uint32_t, t);
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, v2bf));
 }
 
 // Maximum over the four lanes of a column (n, n + 16, n + 32, n + 48).
@@ -193,15 +197,109 @@ __device__ __forceinline__ float col_max(float x) {
   return pair_max(x);
 }
 
-// Range of a row tile's keys: [lo, hi] of one query position of sequence length `len`.
-__device__ __forceinline__ void kv4_limits(const Kv4AttnArgs& a, int len, int pos0, int i, int& lo, int& hi) {
-  const int qpos = pos0 + i;
-  hi = a.causal ? min(len - 1, qpos) : len - 1;
-  lo = a.window > 0 ? max(0, qpos - a.window + 1) : 0;
+// The keys that query i of a sequence sees: [lo, hi].
+struct Kv4Seq {
+  int len, pos0;
+};
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b) {
+  Kv4Seq s;
+  s.len = a.kv_len ? min(max(a.kv_len[b], 0), a.Sk) : a.Sk;
+  s.pos0 = a.kv_len ? s.len - a.Sq : a.q_pos0;
+  return s;
+}
+__device__ __forceinline__ void kv4_limits(const Kv4AttnArgs& a, Kv4Seq s, int i, int& lo, int& hi) {
+  hi = a.causal ? min(s.len - 1, s.pos0 + i) : s.len - 1;
+  lo = a.window > 0 ? max(0, s.pos0 + i - a.window + 1) : 0;
+}
+
+// Items are (sequence, row tile, KV head), the heads fastest; `gt` = sequence * n_rt + row tile.  First and last
+// query of a row tile, and the 64-key blocks that its items walk (the first query sees the lowest key, the last
+// the highest).
+__device__ __forceinline__ void kv4_tile(const Kv4AttnArgs& a, int gt, int& b, int& row0, int& i0, int& i1) {
+  b = a.n_rt == 1 ? gt : gt / a.n_rt;
+  row0 = a.n_rt == 1 ? 0 : (gt - b * a.n_rt) * a.tile_rows;
+  i0 = a.n_rt == 1 ? 0 : row0 / a.group;
+  i1 = a.n_rt == 1 ? a.Sq - 1 : (min(row0 + a.tile_rows, a.rows) - 1) / a.group;
+}
+__device__ __forceinline__ int kv4_blocks(const Kv4AttnArgs& a, int gt) {
+  int b, row0, i0, i1, lo, hi, t;
+  kv4_tile(a, gt, b, row0, i0, i1);
+  const Kv4Seq s = kv4_seq(a, b);
+  kv4_limits(a, s, i0, lo, t);
+  kv4_limits(a, s, i1, t, hi);
+  return hi >= lo ? hi / KV4_BK - lo / KV4_BK + 1 : 1;
+}
+// What an item takes up in the line: its blocks and, short ones, room for the time that a piece costs by itself
+// (Q, the first loads, the merge: some 8 blocks' worth), so that a share does not hold many of them.
+__device__ __forceinline__ int kv4_room(int nblk) { return nblk < 32 ? nblk + 8 : nblk; }
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k);
+  return x;
+}
+// Share of a workgroup for a line of `total`.
+__device__ __forceinline__ int kv4_share(const Kv4AttnArgs& a, int total) {
+  const int s = (total + a.n_wg - 1) / a.n_wg;
+  return max((s + KV4_NW - 1) / KV4_NW * KV4_NW, a.min_share);
+}
+// Room of the items of row tiles before g_end.
+__device__ __forceinline__ int kv4_line(const Kv4AttnArgs& a, int lane, int g_end) {
+  int n = 0;
+  for (int gt = lane; gt < g_end; gt += 64) n += kv4_room(kv4_blocks(a, gt));
+  return __builtin_amdgcn_readfirstlane(wave_sum(n)) * a.Hkv;
+}
+
+// Places u0 .. u1 - 1 of the line are this workgroup's: row tile gt, `in` into its items.  False: none.
+__device__ __forceinline__ bool kv4_my_share(const Kv4AttnArgs& a, int lane, int& u0, int& u1, int& gt, int& in) {
+  if (!a.n_wg) {                           // one workgroup per item, the tiles that see most keys first
+    gt = a.B * a.n_rt - 1 - blockIdx.x / a.Hkv;
+    u0 = 0;
+    u1 = kv4_room(kv4_blocks(a, gt));
+    in = blockIdx.x % a.Hkv * u1;
+    return true;
+  }
+  const int groups = a.B * a.n_rt;
+  int mine = lane < groups ? kv4_room(kv4_blocks(a, lane)) * a.Hkv : 0, sum = mine;
+  auto prefix = [&] {                      // inclusive
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const int x = __shfl_up(sum, k);
+      sum += lane >= k ? x : 0;
+    }
+  };
+  prefix();
+  const int total = groups <= 64 ? __builtin_amdgcn_readlane(sum, 63) : kv4_line(a, lane, groups);
+  const int share = kv4_share(a, total);
+  u0 = blockIdx.x * share;
+  if (u0 >= total) return false;
+  u1 = min(total, u0 + share);
+  for (int g0 = 0, at = 0;;) {             // at: places before tile g0
+    const uint64_t past = __ballot(at + sum > u0);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      gt = g0 + l;
+      in = u0 - (at + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
+      return true;
+    }
+    at += __builtin_amdgcn_readlane(sum, 63);
+    g0 += 64;
+    sum = mine = g0 + lane < groups ? kv4_room(kv4_blocks(a, g0 + lane)) * a.Hkv : 0;
+    prefix();
+  }
+}
+
+// Row r of a KV head's O: 4 values from d on, or (a piece of an item) to the workspace.
+__device__ __forceinline__ void kv4_store4(const Kv4AttnArgs& a, int b, int kvh, int r, int d, float4 x) {
+  const int64_t o = b * a.o_b + (kvh * a.group + r % a.group) * a.o_h + r / a.group * a.o_t + d;
+  if (a.o_bf16)
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + o) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
+  else
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.o) + o) = x;
 }
 
 // PT: bf16 terms of P in the PV product.
-template <int D, bool SOFTCAP, int PT>
+template <int D, int NT, bool SOFTCAP, int PT>
 __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
   constexpr int NW = KV4_NW, BK = KV4_BK;
   constexpr int KD = D / 32;             // K dwords of a lane and row: MFMAs of the score
@@ -213,311 +311,705 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
   __shared__ float sml[NW][16][2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int part = blockIdx.x % a.n_parts, item = blockIdx.x / a.n_parts;
-  const int rt = item % a.n_rt, bk = item / a.n_rt;
-  const int b = bk / a.Hkv, kvh = bk % a.Hkv;
-  const int len = a.kv_len ? min(max(a.kv_len[b], 0), a.Sk) : a.Sk;
-  const int pos0 = a.kv_len ? len - a.Sq : a.q_pos0;
-  const int row0 = rt * 16, row = row0 + n, nrow = min(16, a.rows - row0);
-  const bool valid = n < nrow;
-  const int qi = (valid ? row : row0) / a.group, hd = kvh * a.group + (valid ? row : row0) % a.group;
 
-  // this column's keys, and those that every column of the tile sees or any does
-  int klo, khi, klo_all, khi_all, klo_any, khi_any;
-  kv4_limits(a, len, pos0, qi, klo, khi);
-  kv4_limits(a, len, pos0, row0 / a.group, klo_any, khi_all);
-  kv4_limits(a, len, pos0, (row0 + nrow - 1) / a.group, klo_all, khi_any);
+  int u0, u1, gt, in;
+  if (!kv4_my_share(a, lane, u0, u1, gt, in)) return;
+  bool first = true;
 
-  // Q: column n, k of MFMA kk: d = qd(kk) + e
-  v4i q[KD];
-  const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_b + hd * a.q_h + qi * a.q_t;
+  while (true) {
+    const int nblk = kv4_blocks(a, gt), room = kv4_room(nblk), b = gt;       // (one row tile)
+    const int kvh = in / room, j0 = in - kvh * room, take = min(room - j0, u1 - u0), nj = min(nblk - j0, take);
+    if (nj > 0) {
+    const int bk = b * a.Hkv + kvh;
+    const Kv4Seq seq = kv4_seq(a, b);
+    // each column's keys, and those that every column sees or any does
+    int klo[NT], khi[NT], klo_all, khi_all, klo_any, khi_any;
+    kv4_limits(a, seq, 0, klo_any, khi_all);
+    kv4_limits(a, seq, a.Sq - 1, klo_all, khi_any);
+    // Q: column n, k of MFMA kk: d = qd(kk) + e
+    v4i q[NT][KD];
 #pragma unroll
-  for (int kk = 0; kk < KD; kk++) {
-    const int d = D == 256 ? (kk >> 2) * 128 + g * 32 + 8 * (kk & 3) : g * (D / 4) + 8 * kk;
-    q[kk] = valid ? *reinterpret_cast<const v4i*>(qp + d) : (v4i){0, 0, 0, 0};
-  }
-
-  const int64_t bytes = (int64_t)a.L * (D / 2), sbytes = (int64_t)a.L * NB;
-  const __amdgpu_buffer_rsrc_t rk = buf_rsrc(a.k, bk * bytes, bytes), rv = buf_rsrc(a.v, bk * bytes, bytes);
-  const __amdgpu_buffer_rsrc_t rks = buf_rsrc(a.ks, bk * sbytes, sbytes), rvs = buf_rsrc(a.vs, bk * sbytes, sbytes);
-
-  uint32_t kr[4][KD], ksr[2][D == 256 ? 2 : 1];
-  uint32_t vr[2][8][VB > 4 ? 2 : 1];
-  v2i vsr[2];
-  // A disabled load gets an offset past every resource: it reads nothing and returns 0.
-  auto load_k = [&](int key0, bool on) {
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const int key = key0 + 32 * (t >> 1) + 16 * (t & 1) + 4 * (n & 3) + (n >> 2);
-      const uint32_t o = on ? (uint32_t)(key * (D / 2)) : 0x80000000u;
-      if constexpr (D == 64) {
-        const v2i w = __builtin_amdgcn_raw_buffer_load_b64(rk, o + 8 * g, 0, 0);
-        kr[t][0] = w[0]; kr[t][1] = w[1];
-      } else {
-#pragma unroll
-        for (int c = 0; c < KD / 4; c++) {
-          const v4i w = __builtin_amdgcn_raw_buffer_load_b128(rk, o + 64 * c + 16 * g, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 4; i++) kr[t][4 * c + i] = w[i];
-        }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const uint32_t o = on ? (uint32_t)((key0 / 32 + u) * (32 * NB) + 2 * (n & 3)) : 0x80000000u;
-#pragma unroll
-      for (int c = 0; c < (D == 256 ? 2 : 1); c++)
-        ksr[u][c] = __builtin_amdgcn_raw_buffer_load_b16(rks, o + 8 * ((n >> 2) * NB + (D == 64 ? g >> 1 : 4 * c + g)), 0, 0);
-    }
-  };
-  auto load_v = [&](int key0, bool on) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int key = key0 + 32 * u + 16 * (e >> 2) + 4 * (e & 3) + g;
-        const uint32_t o = on ? (uint32_t)(key * (D / 2) + n * VB) : 0x80000000u;
-        if constexpr (VB == 2)
-          vr[u][e][0] = __builtin_amdgcn_raw_buffer_load_b16(rv, o, 0, 0);
-        else if constexpr (VB == 4)
-          vr[u][e][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, 0, 0);
-        else {
-          const v2i w = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, 0);
-          vr[u][e][0] = w[0]; vr[u][e][1] = w[1];
-        }
-      }
-      const uint32_t o = on ? (uint32_t)((key0 / 32 + u) * (32 * NB) + 8 * (g * NB + n * NB / 16)) : 0x80000000u;
-      vsr[u] = __builtin_amdgcn_raw_buffer_load_b64(rvs, o, 0, 0);
-    }
-  };
-
-  v4f o[ND];
-#pragma unroll
-  for (int j = 0; j < ND; j++) o[j] = (v4f){0, 0, 0, 0};
-  float mc = -INFINITY, l = 0.0f;
-  const float c = SOFTCAP ? 1.0f : a.c_log2;
-
-  // blocks of this wave: first, first + step, ... while their first key is at most khi_any
-  const int step = a.n_parts * NW * BK;
-  const int kfirst = (klo_any / BK + part * NW + wave) * BK;
-  load_k(kfirst, kfirst <= khi_any);
-  load_v(kfirst, kfirst <= khi_any);
-  for (int key0 = kfirst; key0 <= khi_any; key0 += step) {
-    const bool more = key0 + step <= khi_any;
-    // ---- S^T
-    v4f s[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-      s[t] = (v4f){0, 0, 0, 0};
+    for (int t = 0; t < NT; t++) {
+      const int row = 16 * t + n;
+      const bool valid = row < a.rows;
+      const int qi = valid ? row / a.group : 0, hd = kvh * a.group + (valid ? row % a.group : 0);
+      kv4_limits(a, seq, qi, klo[t], khi[t]);
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_b + hd * a.q_h + qi * a.q_t;
 #pragma unroll
       for (int kk = 0; kk < KD; kk++) {
-        const float sc = scale_byte(ksr[t >> 1][D == 256 ? kk >> 2 : 0], t & 1);
-        v4i ka;
-#pragma unroll
-        for (int i = 0; i < 4; i++) ka[i] = (int)cvt_fp4_bf16(kr[t][kk], sc, i);
-        s[t] = mfma16(ka, q[kk], s[t]);
+        const int d = D == 256 ? (kk >> 2) * 128 + g * 32 + 8 * (kk & 3) : g * (D / 4) + 8 * kk;
+        q[t][kk] = valid ? *reinterpret_cast<const v4i*>(qp + d) : (v4i){0, 0, 0, 0};
       }
     }
-    load_k(key0 + step, more);
-    if (SOFTCAP) {
+
+    const int64_t bytes = (int64_t)a.L * (D / 2), sbytes = (int64_t)a.L * NB;
+    const __amdgpu_buffer_rsrc_t rk = buf_rsrc(a.k, bk * bytes, bytes), rv = buf_rsrc(a.v, bk * bytes, bytes);
+    const __amdgpu_buffer_rsrc_t rks = buf_rsrc(a.ks, bk * sbytes, sbytes), rvs = buf_rsrc(a.vs, bk * sbytes, sbytes);
+
+    // Codes are read once, whole lines per instruction: non-temporal loads (64 x 8,192 tokens of D = 128:
+    // 96 us, 104 with the default policy).
+    constexpr int kNT = 2;
+    uint32_t kr[4][KD], ksr[2][D == 256 ? 2 : 1];
+    uint32_t vr[2][8][VB > 4 ? 2 : 1];
+    v2i vsr[2];
+    // (Loads from key L on lie past the resources: they read nothing and return 0.)
+    const uint32_t klane = (4 * (n & 3) + (n >> 2)) * (D / 2) + (D == 64 ? 8 : 16) * g, vlane = g * (D / 2) + n * VB;
+    const uint32_t kslane = 2 * (n & 3) + 8 * ((n >> 2) * NB + (D == 64 ? g >> 1 : g)), vslane = 8 * (g * NB + n * NB / 16);
+    auto load_k = [&](int key0) {
+      const uint32_t base = klane + (uint32_t)key0 * (D / 2), sbase = kslane + (uint32_t)key0 * NB;
 #pragma unroll
-      for (int t = 0; t < 4; t++)
+      for (int t = 0; t < 4; t++) {
+        const uint32_t o = base + 16 * t * (D / 2);
+        if constexpr (D == 64) {
+          const v2i w = __builtin_amdgcn_raw_buffer_load_b64(rk, o, 0, kNT);
+          kr[t][0] = w[0]; kr[t][1] = w[1];
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float u = s[t][i] * a.sc_u;
-          const float e = __builtin_amdgcn_exp2f(-2.0f * LOG2E_F * fabsf(u));
-          const float th = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
-          s[t][i] = a.cap_log2 * (u < 0.0f ? -th : th);
+          for (int c = 0; c < KD / 4; c++) {
+            const v4i w = __builtin_amdgcn_raw_buffer_load_b128(rk, o + 64 * c, 0, kNT);
+#pragma unroll
+            for (int i = 0; i < 4; i++) kr[t][4 * c + i] = w[i];
+          }
         }
-    }
-    if (key0 < klo_all || key0 + BK - 1 > khi_all) {
-      // masked scores to -inf; the scales of V rows that no query of the tile may see (what lies there may
-      // be anything) to 2^-127, so that their product with P = 0 is 0
-#pragma unroll
-      for (int t = 0; t < 4; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int key = key0 + 16 * t + 4 * i + g;
-          s[t][i] = key >= klo && key <= khi ? s[t][i] : -INFINITY;
-        }
+      }
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
+        for (int c = 0; c < (D == 256 ? 2 : 1); c++)
+          ksr[u][c] = __builtin_amdgcn_raw_buffer_load_b16(rks, sbase + 32 * NB * u + 32 * c, 0, 0);
+    };
+    auto load_v = [&](int key0) {
+      const uint32_t base = vlane + (uint32_t)key0 * (D / 2), sbase = vslane + (uint32_t)key0 * NB;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+#pragma unroll
         for (int e = 0; e < 8; e++) {
-          const int by = 2 * (e & 3) + (e >> 2);
-          const int key = key0 + 32 * u + 16 * (e >> 2) + 4 * (e & 3) + g;
-          if (key < klo_any || key > khi_any) vsr[u][by >> 2] &= ~(0xff << (8 * (by & 3)));
+          const uint32_t o = base + (32 * u + 16 * (e >> 2) + 4 * (e & 3)) * (D / 2);
+          if constexpr (VB == 2)
+            vr[u][e][0] = __builtin_amdgcn_raw_buffer_load_b16(rv, o, 0, kNT);
+          else if constexpr (VB == 4)
+            vr[u][e][0] = __builtin_amdgcn_raw_buffer_load_b32(rv, o, 0, kNT);
+          else {
+            const v2i w = __builtin_amdgcn_raw_buffer_load_b64(rv, o, 0, kNT);
+            vr[u][e][0] = w[0]; vr[u][e][1] = w[1];
+          }
         }
+        vsr[u] = __builtin_amdgcn_raw_buffer_load_b64(rvs, sbase + 32 * NB * u, 0, 0);
+      }
+    };
+
+    v4f o[NT][ND];
+    float mc[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+#pragma unroll
+      for (int j = 0; j < ND; j++) o[t][j] = (v4f){0, 0, 0, 0};
+      mc[t] = -INFINITY;
+      l[t] = 0.0f;
     }
-    // ---- reference exponent
-    float mx = s[0][0];
-#pragma unroll
-    for (int t = 0; t < 4; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][i]);
-    if (__any(__builtin_fmaf(mx, c, -mc) > kSlack)) {
-      // (by the column's own maximum: a row's result does not depend on its neighbours in the tile)
-      const float top = col_max(mx);
-      const bool up = __builtin_fmaf(top, c, -mc) > kSlack;
-      const float corr = up ? __builtin_amdgcn_exp2f(mc - top * c) : 1.0f;
-      mc = up ? top * c : mc;
-      l *= corr;
-#pragma unroll
-      for (int j = 0; j < ND; j++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) o[j][i] *= corr;
-    }
-    const float mcn = mc == -INFINITY ? 0.0f : -mc;
-    // ---- P: its terms as B operands of the two 32-key products
-    v4i p[2][PT];
-#pragma unroll
-    for (int u = 0; u < 2; u++)
+    const float c = SOFTCAP ? 1.0f : a.c_log2;
+
+    // this wave's blocks: every NW-th of the piece's nj, from block j0 of the item on
+    const int kend = (klo_any / BK + j0 + nj) * BK, kfirst = (klo_any / BK + j0 + wave) * BK;
+    // (in this order, as in the loop: the wait for K must not become one for V)
+    load_k(kfirst < kend ? kfirst : a.L);
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(kfirst < kend ? kfirst : a.L);
+    __builtin_amdgcn_sched_barrier(0);
+    for (int key0 = kfirst; key0 < kend; key0 += NW * BK) {
+      const int next = key0 + NW * BK < kend ? key0 + NW * BK : a.L;
+      const bool masked = key0 < klo_all || key0 + BK - 1 > khi_all;
+      // ---- S^T
+      v4f s[NT][4];
 #pragma unroll
       for (int x = 0; x < 4; x++) {
-        const int t = 2 * u + (x >> 1), i = 2 * (x & 1);
-        float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], c, mcn));
-        float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i + 1], c, mcn));
-        if constexpr (PT > 1) l += p0 + p1;
 #pragma unroll
-        for (int y = 0; y < PT; y++) {
-          const uint32_t w = pack_bf16(p0, p1);
-          p[u][y][x] = (int)w;
-          const float r0 = __uint_as_float(w << 16), r1 = __uint_as_float(w & 0xffff0000u);
-          if constexpr (PT == 1) l += r0 + r1;
-          p0 -= r0;
-          p1 -= r1;
+        for (int t = 0; t < NT; t++) s[t][x] = (v4f){0, 0, 0, 0};
+#pragma unroll
+        for (int kk = 0; kk < KD; kk++) {
+          const float sc = scale_byte(ksr[x >> 1][D == 256 ? kk >> 2 : 0], x & 1);
+          v4i ka;
+#pragma unroll
+          for (int i = 0; i < 4; i++) ka[i] = (int)cvt_fp4_bf16(kr[x][kk], sc, i);
+#pragma unroll
+          for (int t = 0; t < NT; t++) s[t][x] = mfma16(ka, q[t][kk], s[t][x]);
         }
       }
-    // ---- O^T += V^T P^T
+      load_k(next);
+      v4i p[NT][2][PT];                    // P's terms, B operands of the two 32-key products
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-      float sc[8];
+      for (int t = 0; t < NT; t++) {
+        if (SOFTCAP) {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int by = 2 * (e & 3) + (e >> 2);
-        sc[e] = scale_byte((uint32_t)vsr[u][by >> 2], by & 3);
+          for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float u = s[t][x][i] * a.sc_u;
+              const float e = __builtin_amdgcn_exp2f(-2.0f * LOG2E_F * fabsf(u));
+              const float th = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+              s[t][x][i] = a.cap_log2 * (u < 0.0f ? -th : th);
+            }
+        }
+        if (masked) {
+          __asm__ volatile("");            // (keeps the selects behind the branch)
+#pragma unroll
+          for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int key = key0 + 16 * x + 4 * i + g;
+              s[t][x][i] = key >= klo[t] && key <= khi[t] ? s[t][x][i] : -INFINITY;
+            }
+        }
+        // ---- reference exponent
+        float mx = s[t][0][0];
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) mx = fmaxf(mx, s[t][x][i]);
+        if (__any(__builtin_fmaf(mx, c, -mc[t]) > kSlack)) {
+          // (by the column's own maximum: a row's result does not depend on its neighbours in the tile)
+          const float top = col_max(mx);
+          const bool up = __builtin_fmaf(top, c, -mc[t]) > kSlack;
+          const float corr = up ? __builtin_amdgcn_exp2f(mc[t] - top * c) : 1.0f;
+          mc[t] = up ? top * c : mc[t];
+          l[t] *= corr;
+#pragma unroll
+          for (int j = 0; j < ND; j++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[t][j][i] *= corr;
+        }
+        const float mcn = mc[t] == -INFINITY ? 0.0f : -mc[t];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            const int tt = 2 * u + (x >> 1), i = 2 * (x & 1);
+            float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][tt][i], c, mcn));
+            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][tt][i + 1], c, mcn));
+            l[t] += p0 + p1;
+#pragma unroll
+            for (int y = 0; y < PT; y++) {
+              const uint32_t w = pack_bf16(p0, p1);
+              p[t][u][y][x] = (int)w;
+              p0 -= __uint_as_float(w << 16);
+              p1 -= __uint_as_float(w & 0xffff0000u);
+            }
+          }
+      }
+      // ---- O^T += V^T P^T
+      uint32_t vw[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) vw[u][i] = (uint32_t)vsr[u][i];
+      if (masked) {
+        // the scales of V rows that no query may see (what lies there may be anything) to 2^-127, so
+        // that their product with P = 0 is 0
+        __asm__ volatile("");
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const int by = 2 * (e & 3) + (e >> 2), key = key0 + 32 * u + 16 * (e >> 2) + 4 * (e & 3) + g;
+            if (key < klo_any || key > khi_any) vw[u][by >> 2] &= ~(0xffu << (8 * (by & 3)));
+          }
       }
 #pragma unroll
-      for (int by = 0; by < VB; by++) {
-        uint32_t w[8];
+      for (int u = 0; u < 2; u++) {
+        float sc[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = cvt_fp4_bf16(vr[u][e][by >> 2], sc[e], by & 3);
-        v4i v0, v1;
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-          v0[x] = (int)__builtin_amdgcn_perm(w[2 * x + 1], w[2 * x], 0x05040100u);
-          v1[x] = (int)__builtin_amdgcn_perm(w[2 * x + 1], w[2 * x], 0x07060302u);
+        for (int e = 0; e < 8; e++) {
+          const int by = 2 * (e & 3) + (e >> 2);
+          sc[e] = scale_byte(vw[u][by >> 2], by & 3);
         }
 #pragma unroll
-        for (int y = 0; y < PT; y++) {
-          o[2 * by] = mfma16(v0, p[u][y], o[2 * by]);
-          o[2 * by + 1] = mfma16(v1, p[u][y], o[2 * by + 1]);
+        for (int by = 0; by < VB; by++) {
+          uint32_t w[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) w[e] = cvt_fp4_bf16(vr[u][e][by >> 2], sc[e], by & 3);
+          v4i v0, v1;
+#pragma unroll
+          for (int x = 0; x < 4; x++) {
+            v0[x] = (int)__builtin_amdgcn_perm(w[2 * x + 1], w[2 * x], 0x05040100u);
+            v1[x] = (int)__builtin_amdgcn_perm(w[2 * x + 1], w[2 * x], 0x07060302u);
+          }
+#pragma unroll
+          for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int y = 0; y < PT; y++) {
+              o[t][2 * by] = mfma16(v0, p[t][u][y], o[t][2 * by]);
+              o[t][2 * by + 1] = mfma16(v1, p[t][u][y], o[t][2 * by + 1]);
+            }
         }
       }
+      load_v(next);
     }
-    load_v(key0 + step, more);
-  }
 
-  // ---- merge the waves: d = (4 g + i) ND + j of column n
-  l += __shfl_xor(l, 16);
-  l = pair_sum(l);
+    // ---- merge the waves, a tile of columns at a time: d = (4 g + i) ND + j of column n
+    const bool whole = nj == nblk;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+    for (int t = 0; t < NT; t++) {
+      l[t] += __shfl_xor(l[t], 16);
+      l[t] = pair_sum(l[t]);
+      __syncthreads();                     // (the tile of the last merge has been read)
 #pragma unroll
-    for (int j = 0; j < ND; j += 4)
-      *reinterpret_cast<float4*>(&so[wave][n][(4 * g + i) * ND + j]) = make_float4(o[j][i], o[j + 1][i], o[j + 2][i], o[j + 3][i]);
-  if (g == 0) {
-    sml[wave][n][0] = mc;
-    sml[wave][n][1] = l;
-  }
-  __syncthreads();
-  // thread (col, x) = (tid / 16, tid % 16): 4 consecutive d at 4 x, 4 x + 64, ...
-  const int col = tid >> 4, d0 = 4 * (tid & 15);
-  if (col >= nrow) return;
-  float M = -INFINITY, L = 0.0f, wt[NW];
+      for (int i = 0; i < 4; i++)
 #pragma unroll
-  for (int w = 0; w < NW; w++) M = fmaxf(M, sml[w][col][0]);
+        for (int j = 0; j < ND; j += 4)
+          *reinterpret_cast<float4*>(&so[wave][n][(4 * g + i) * ND + j]) =
+              make_float4(o[t][j][i], o[t][j + 1][i], o[t][j + 2][i], o[t][j + 3][i]);
+      if (g == 0) {
+        sml[wave][n][0] = mc[t];
+        sml[wave][n][1] = l[t];
+      }
+      __syncthreads();
+      // thread (col, x) = (tid / 16, tid % 16): 4 consecutive d at 4 x, 4 x + 64, ...
+      const int col = tid >> 4, d0 = 4 * (tid & 15), r = 16 * t + col;
+      if (r >= a.rows) continue;
+      float M = -INFINITY, Ls = 0.0f, wt[NW];
 #pragma unroll
-  for (int w = 0; w < NW; w++) {
-    wt[w] = __builtin_amdgcn_exp2f(sml[w][col][0] - (M == -INFINITY ? 0.0f : M));
-    L += sml[w][col][1] * wt[w];
-  }
-  const int r = row0 + col;
-  const int64_t pr = ((int64_t)bk * a.rows + r) * a.n_parts + part;
-  const int64_t oo = b * a.o_b + (kvh * a.group + r % a.group) * a.o_h + r / a.group * a.o_t;
+      for (int w = 0; w < NW; w++) M = fmaxf(M, sml[w][col][0]);
 #pragma unroll
-  for (int d = d0; d < D; d += 64) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 0; w < NW; w++) {
+        wt[w] = __builtin_amdgcn_exp2f(sml[w][col][0] - (M == -INFINITY ? 0.0f : M));
+        Ls += sml[w][col][1] * wt[w];
+      }
+      const float inv = !whole ? 1.0f : Ls != 0.0f ? 1.0f / Ls : 0.0f;   // no visible key: 0
 #pragma unroll
-    for (int w = 0; w < NW; w++) {
-      const float4 x = *reinterpret_cast<const float4*>(&so[w][col][d]);
-      acc.x += x.x * wt[w]; acc.y += x.y * wt[w]; acc.z += x.z * wt[w]; acc.w += x.w * wt[w];
+      for (int d = d0; d < D; d += 64) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+          const float4 x = *reinterpret_cast<const float4*>(&so[w][col][d]);
+          acc.x += x.x * wt[w]; acc.y += x.y * wt[w]; acc.z += x.z * wt[w]; acc.w += x.w * wt[w];
+        }
+        acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
+        if (!whole)
+          *reinterpret_cast<float4*>(a.part_o + (slot * a.tile_rows + r) * D + d) = acc;
+        else
+          kv4_store4(a, b, kvh, r, d, acc);
+      }
+      if (!whole && d0 == 0) reinterpret_cast<float2*>(a.part_ml)[slot * a.tile_rows + r] = make_float2(M, Ls);
     }
-    if (a.n_parts > 1) {
-      *reinterpret_cast<float4*>(a.part_o + pr * D + d) = acc;
-    } else {
-      const float inv = L != 0.0f ? 1.0f / L : 0.0f;             // no visible key: 0
-      acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
-      if (a.o_bf16)
-        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + oo + d) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
-      else
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.o) + oo + d) = acc;
     }
-  }
-  if (a.n_parts > 1 && d0 == 0) {
-    a.part_ml[2 * pr] = M;
-    a.part_ml[2 * pr + 1] = L;
+    u0 += take;
+    if (u0 >= u1) return;
+    first = false;
+    in += take;
+    if (in == room * a.Hkv) {
+      in = 0;
+      gt++;
+    }
   }
 }
 
-#define MXFA_KV4_ATTN(D, SC, PT, NAME) \
-  extern "C" __global__ void __launch_bounds__(256, 2) NAME(Kv4AttnArgs a) { kv4_attn_impl<D, SC, PT>(a); }
-#define MXFA_KV4_ATTN_ALL(D)                                            \
-  MXFA_KV4_ATTN(D, false, 2, mxfa_kv4_attn_d##D)                        \
-  MXFA_KV4_ATTN(D, true, 2, mxfa_kv4_attn_d##D##_softcap)               \
-  MXFA_KV4_ATTN(D, false, 3, mxfa_kv4_attn_d##D##_f32)                  \
-  MXFA_KV4_ATTN(D, true, 3, mxfa_kv4_attn_d##D##_softcap_f32)
-MXFA_KV4_ATTN_ALL(64)
-MXFA_KV4_ATTN_ALL(128)
-MXFA_KV4_ATTN_ALL(256)
+#define MXFA_KV4_ATTN(D, NT, SC, PT, OCC, NAME) \
+  extern "C" __global__ void __launch_bounds__(64 * KV4_NW, OCC) NAME(Kv4AttnArgs a) { kv4_attn_impl<D, NT, SC, PT>(a); }
+#define MXFA_KV4_ATTN_ALL(D, NT, OCC)                                           \
+  MXFA_KV4_ATTN(D, NT, false, 2, OCC, mxfa_kv4_attn_d##D##_t##NT)               \
+  MXFA_KV4_ATTN(D, NT, true, 2, OCC, mxfa_kv4_attn_d##D##_t##NT##_softcap)      \
+  MXFA_KV4_ATTN(D, NT, false, 3, OCC, mxfa_kv4_attn_d##D##_t##NT##_f32)         \
+  MXFA_KV4_ATTN(D, NT, true, 3, OCC, mxfa_kv4_attn_d##D##_t##NT##_softcap_f32)
+MXFA_KV4_ATTN_ALL(64, 1, 2)
+MXFA_KV4_ATTN_ALL(64, 2, 2)
+MXFA_KV4_ATTN_ALL(128, 1, 2)
+MXFA_KV4_ATTN_ALL(128, 2, 2)
+MXFA_KV4_ATTN_ALL(256, 1, 2)
+MXFA_KV4_ATTN_ALL(256, 2, 1)
 
-// O = sum_p O_p 2^(m_p - M) / sum_p l_p 2^(m_p - M) of the parts of each row; 0 where nothing was visible.
-// One workgroup of D threads per row, D / 4 lanes of 4 d for each of 4 groups that take every fourth part.
+// ---------------------------------------------------------------------------
+// Attention, tiled form: more than 32 query rows of a KV head.  128 rows to a workgroup (32 to each of its four
+// waves), 64 keys at a time: the workgroup widens the block's K and V to bf16 (exact) in LDS once, and every
+// wave takes S^T = K Q^T and O^T += V^T P^T over its own rows on the 32x32x16 bf16 MFMA, both A operands read
+// from LDS.  Lane (n, h) = (lane % 32, lane / 32):
+//   A operand: row n, k = 8 h + e (e < 8); B: column n, k likewise; C: column n, rows 8 (i / 4) + 4 h + i % 4.
+// V lies transposed, a row of 64 keys for each d, the keys of a 16-key group in the order in which a lane
+// holds their scores (8 h + e is key 8 (e / 4) + 4 h + e % 4), so P goes from the score's registers into
+// the B operand as it is.  LDS rows are cut into 16-byte units, unit u of K row `key` at u ^ (key & 15) (D = 256:
+// the upper 16 units at u ^ ((key ^ 8) & 15); D = 64, rows of 8: u ^ ((key ^ key / 8) & 7)), of V row d, 8 units, at u ^
+// ((d ^ d / 8) & 7) of row d ^ (d / 64 & 1): reads and writes of 16 consecutive lanes hit distinct banks.
+//
+// What bounds it: the MFMAs (33 clocks each) and about as many clocks of 4- and 8-clock VALU work (exponentials,
+// conversions), which run beside MFMAs only if an instruction stream has both.  So the scores run a block ahead:
+// the MFMAs of block j + 1's scores go between the exponentials of block j, those of block j's PV product
+// between the widening of K of block j + 2 and V of block j + 1, whose codes were loaded an iteration before; two
+// buffers each, one barrier per block.
+// Softmax as in the streaming form, and the same line of items, here with row tiles.
+// ---------------------------------------------------------------------------
+// PT: bf16 terms of P in the PV product.
+template <int D, bool SOFTCAP, int PT>
+__device__ __forceinline__ void kv4_tiled_impl(const Kv4AttnArgs& a) {
+  constexpr int BK = KV4_BK, NB = D / 32, ND = D / 32;
+  constexpr int TW = D == 256 ? 2 : 1;     // pieces of K (an MX block) and of V (4 keys x 8 d) that a thread widens
+  constexpr int BUF = BK * D * 2;          // bytes of a block's K, and of its V
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * BUF];   // K, K, V, V
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  int u0, u1, gt, in;
+  if (!kv4_my_share(a, lane, u0, u1, gt, in)) return;
+  bool first = true;
+
+  while (true) {
+    const int nblk = kv4_blocks(a, gt), room = kv4_room(nblk);
+    const int kvh = in / room, j0 = in - kvh * room, take = min(room - j0, u1 - u0), nj = min(nblk - j0, take);
+    if (nj > 0) {
+      int b, row0, i0, i1;
+      kv4_tile(a, gt, b, row0, i0, i1);
+      const int bk = b * a.Hkv + kvh;
+      const Kv4Seq seq = kv4_seq(a, b);
+      int klo_any, khi_any, t0, t1;
+      kv4_limits(a, seq, i0, klo_any, t0);
+      kv4_limits(a, seq, i1, t1, khi_any);
+      // the wave's rows: each column's keys, and those that all of them see (a wave without rows need not mask any)
+      const int wrow0 = row0 + wave * 32, wrow1 = min(wrow0 + 32, a.rows) - 1;
+      int wlo_all = 0, whi_all = INT32_MAX;
+      if (wrow0 < a.rows) {
+        kv4_limits(a, seq, wrow0 / a.group, t0, whi_all);
+        kv4_limits(a, seq, wrow1 / a.group, wlo_all, t1);
+      }
+      const int row = wrow0 + n;
+      const bool valid = row < a.rows;
+      const int qi = valid ? row / a.group : i0, hd = kvh * a.group + (valid ? row % a.group : 0);
+      int klo, khi;
+      kv4_limits(a, seq, qi, klo, khi);
+      const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_b + hd * a.q_h + qi * a.q_t;
+      v4i q[D / 16];
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk++) q[kk] = valid ? *reinterpret_cast<const v4i*>(qp + 16 * kk + 8 * h) : (v4i){0, 0, 0, 0};
+
+      const int64_t bytes = (int64_t)a.L * (D / 2), sbytes = (int64_t)a.L * NB;
+
+      // ---- staging.  K: block kbl of key kk0 (D = 64: every piece twice; D = 256: key + 32 too).  V: the 4 keys of half
+      // vq % 2 of unit vq / 2, 32 (vq / 8) + 16 (vq / 4 % 2) + 8 (vq % 2) + 4 (vq / 2 % 2) + 0 .. 3, and 8 d from 8 vdc on
+      // (D = 64: every piece twice; D = 256: keys + 32 too).
+      // (Loads from key L on lie past the resources: they read nothing and return 0.)
+      uint32_t kraw[4 * TW], krs[TW], vraw[4 * TW], vrs[4 * TW];
+      const int kbl = tid % NB, kk0 = tid / NB & 63, vdc = (tid >> 1) % (D / 8), vq = 2 * (tid / (D / 4) & 7) + (tid & 1);
+      const int vk0 = 32 * (vq >> 3) + 16 * ((vq >> 2) & 1) + 8 * (vq & 1) + 4 * ((vq >> 1) & 1);
+      const uint32_t klb = kk0 * (D / 2) + 16 * kbl;
+      const uint32_t vlb = vk0 * (D / 2) + 4 * vdc;
+      // scales: byte x of a group's 8, read as the dword that holds it and turned so that it lies in a float's exponent
+      // (a byte load's value would be looked at, to extend it, before it is used, and waited for)
+      const uint32_t kx = 2 * ((kk0 >> 2) & 3) + ((kk0 >> 4) & 1), vx = 2 * ((vk0 >> 2) & 3) + ((vk0 >> 4) & 1);
+      const uint32_t kls = (kk0 >> 5) * (32 * NB) + ((kk0 & 3) * NB + kbl) * 8 + (kx & 4), kturn = 8 * (kx & 3) + 9 & 31;
+      const uint32_t vls = (vk0 >> 5) * (32 * NB) + (vdc >> 2) * 8 + (vx & 4), vturn = 8 * (vx & 3) + 9 & 31;
+      auto turned = [](uint32_t w, uint32_t by) { return __uint_as_float(__builtin_amdgcn_alignbit(w, w, by)); };
+      // (the block's place goes into the resource, by the scalar unit: a thread's offsets stay the same)
+      const uint8_t *kbase = a.k + bk * bytes, *vbase = a.v + bk * bytes, *ksbase = a.ks + bk * sbytes, *vsbase = a.vs + bk * sbytes;
+      auto from = [&](const uint8_t* base, int key0, int per) {   // (key0 <= L, L * per < 2^31)
+        return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (uint32_t)(key0 * per)), 0, (a.L - key0) * per, 0x00020000);
+      };
+      auto load_k = [&](int key0) {
+        const __amdgpu_buffer_rsrc_t r = from(kbase, key0, D / 2), rs = from(ksbase, key0, NB);
+#pragma unroll
+        for (int v = 0; v < TW; v++) {
+          const v4i w = __builtin_amdgcn_raw_buffer_load_b128(r, klb + 32 * v * (D / 2), 0, 0);
+#pragma unroll
+          for (int x = 0; x < 4; x++) kraw[4 * v + x] = (uint32_t)w[x];
+          krs[v] = __builtin_amdgcn_raw_buffer_load_b32(rs, kls + 32 * v * NB, 0, 0);
+        }
+      };
+      auto load_v = [&](int key0) {
+        const __amdgpu_buffer_rsrc_t r = from(vbase, key0, D / 2), rs = from(vsbase, key0, NB);
+#pragma unroll
+        for (int i = 0; i < 4 * TW; i++) {
+          vraw[i] = __builtin_amdgcn_raw_buffer_load_b32(r, vlb + (32 * (i >> 2) + (i & 3)) * (D / 2), 0, 0);
+          vrs[i] = __builtin_amdgcn_raw_buffer_load_b32(rs, vls + (i >> 2) * (32 * NB) + (i & 3) * (8 * NB), 0, 0);
+        }
+      };
+      // V rows of the block at key0 that no query of the tile may see (what lies there may be anything) get scale 2^-127,
+      // so that their product with P = 0 is 0
+      auto hide_v = [&](int key0) {
+        if (key0 < klo_any || key0 + BK - 1 > khi_any) {
+          __asm__ volatile("");
+#pragma unroll
+          for (int i = 0; i < 4 * TW; i++) {
+            const int key = key0 + vk0 + 32 * (i >> 2) + (i & 3);
+            vrs[i] = key < klo_any || key > khi_any ? 0u : vrs[i];
+          }
+        }
+      };
+      // (a unit's place in a row is its number XOR the row's swizzle: rows are aligned to their length)
+      uint32_t kst = kk0 * (2 * D) + (kbl >> 2) * 256 +
+                     (((D == 64 ? (kk0 ^ (kk0 >> 3)) & 7 : (kk0 ^ 8 * (kbl >> 2)) & 15) ^ (4 * (kbl & 3))) << 4);
+      uint32_t vst = 2 * BUF + vdc * 1024 + 128 * ((vdc >> 3) & 1) + (((vq >> 1) ^ (vdc & 7)) << 4) + 8 * (vq & 1);
+      auto stage_k = [&](int v, int x) {       // 8 elements of piece v
+        v4i w;
+#pragma unroll
+        for (int y = 0; y < 4; y++) w[y] = (int)cvt_fp4_bf16(kraw[4 * v + x], turned(krs[v], kturn), y);
+        *reinterpret_cast<v4i*>(lds + (kst ^ 16 * x) + v * (64 * D)) = w;
+      };
+      auto stage_v = [&](int v, int by) {      // 2 of the 8 d of piece v
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = cvt_fp4_bf16(vraw[4 * v + e], turned(vrs[4 * v + e], vturn), by);
+        const v2i x0 = {(int)__builtin_amdgcn_perm(w[1], w[0], 0x05040100u), (int)__builtin_amdgcn_perm(w[3], w[2], 0x05040100u)};
+        const v2i x1 = {(int)__builtin_amdgcn_perm(w[1], w[0], 0x07060302u), (int)__builtin_amdgcn_perm(w[3], w[2], 0x07060302u)};
+        *reinterpret_cast<v2i*>(lds + (vst ^ (64 * v) ^ (32 * by)) + 256 * by) = x0;
+        *reinterpret_cast<v2i*>(lds + (vst ^ (64 * v) ^ (32 * by + 16 + 128)) + 256 * by) = x1;
+      };
+      auto stage_all = [&](bool with_v) {
+#pragma unroll
+        for (int u = 0; u < 4 * TW; u++) {
+          stage_k(u >> 2, u & 3);
+          if (with_v) stage_v(u >> 2, u & 3);
+        }
+      };
+      // (the scales are turned where they are used and not where they are loaded: that would wait for them)
+      auto pin = [&] {
+#pragma unroll
+        for (int i = 0; i < TW; i++) __asm__ volatile("" : "+v"(krs[i]));
+#pragma unroll
+        for (int i = 0; i < 4 * TW; i++) __asm__ volatile("" : "+v"(vrs[i]));
+      };
+
+      // LDS addresses of the A operands: unit h of K row n and of V row n; the other units are an XOR away
+      uint32_t kat = n * (2 * D) + ((h ^ (D == 64 ? (n ^ (n >> 3)) & 7 : n & 15)) << 4);
+      uint32_t vat = 2 * BUF + n * 128 + ((h ^ ((n ^ (n >> 3)) & 7)) << 4);
+      auto kfrag = [&](int f) {                // kk = f / 2, keys 32 (f % 2) + n
+        const int kk = f >> 1;
+        // (D = 64: key ^ key / 8 of rows 32 on differs from that of row n in bit 2)
+        const int i = D == 64 ? (kk ^ 2 * (f & 1)) & 3 : (kk ^ (D == 256 && kk >= 8 ? 4 : 0)) & 7;
+        return *reinterpret_cast<const v4i*>(lds + (kat ^ 32 * i) + (kk >> 3) * 256 + (f & 1) * (64 * D));
+      };
+      auto vfrag = [&](int f) {                // keys of m = f / ND, d = 32 (f % ND) + n
+        const int j = f % ND, m = f / ND;
+        return *reinterpret_cast<const v4i*>(lds + (vat ^ (32 * (m ^ 2 * (j & 1)) + 128 * ((j >> 1) & 1))) + j * 4096);
+      };
+      constexpr int NK = D / 8, NV = 4 * ND;   // operands of a block
+
+      v16f o[ND], s[2], t[2];
+      float mc = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int j = 0; j < ND; j++) o[j] = (v16f){};
+      const float c = SOFTCAP ? 1.0f : a.c_log2;
+      const int kbeg = (klo_any / BK + j0) * BK, kend = kbeg + nj * BK;
+      auto at_or_none = [&](int key0) { return key0 < kend ? min(key0, a.L) : a.L; };   // (a position past the cache: none)
+
+      // ---- before the first block: its K and V and the second one's K widened, its scores
+      load_k(at_or_none(kbeg));
+      load_v(at_or_none(kbeg));
+      pin();
+      hide_v(kbeg);
+      stage_all(true);
+      load_k(at_or_none(kbeg + BK));
+      load_v(at_or_none(kbeg + BK));
+      __syncthreads();
+      s[0] = s[1] = (v16f){};
+#pragma unroll
+      for (int f = 0; f < NK; f++) s[f & 1] = mfma_bf16(kfrag(f), q[f >> 1], s[f & 1]);
+      kst ^= BUF;
+      vst ^= BUF;
+      kat ^= BUF;
+      pin();
+      stage_all(false);
+      load_k(at_or_none(kbeg + 2 * BK));
+      kst ^= BUF;
+      __syncthreads();
+
+      auto block = [&](int key0, v16f(&s)[2], v16f(&s2)[2]) {
+        // s: this block's scores, s2: the next one's.  K of the next block at kat, V of this one at vat; K of the one after next goes to
+        // kst, V of the next one to vst.
+        if (SOFTCAP) {
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const float u = s[x][i] * a.sc_u;
+              const float e = __builtin_amdgcn_exp2f(-2.0f * LOG2E_F * fabsf(u));
+              const float th = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
+              s[x][i] = a.cap_log2 * (u < 0.0f ? -th : th);
+            }
+        }
+        if (key0 < wlo_all || key0 + BK - 1 > whi_all) {
+          __asm__ volatile("");                // (keeps the selects behind the branch)
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const int key = key0 + 32 * x + 8 * (i >> 2) + 4 * h + (i & 3);
+              s[x][i] = key >= klo && key <= khi ? s[x][i] : -INFINITY;
+            }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[x][i]);
+        if (__any(__builtin_fmaf(mx, c, -mc) > kSlack)) {
+          const float top = pair_max(mx);
+          const bool up = __builtin_fmaf(top, c, -mc) > kSlack;
+          const float corr = up ? __builtin_amdgcn_exp2f(mc - top * c) : 1.0f;
+          mc = up ? top * c : mc;
+          l *= corr;
+#pragma unroll
+          for (int j = 0; j < ND; j++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[j][i] *= corr;
+        }
+        const float mcn = mc == -INFINITY ? 0.0f : -mc;
+        __asm__ volatile("" : "+v"(kat), "+v"(vat), "+v"(kst), "+v"(vst));   // (the XORs stay here: hoisted, they cost registers)
+
+        // ---- the next block's scores, and between their MFMAs this one's P: its terms as B operands of the four 16-key
+        // products.  (Each step is kept together: left to itself the compiler puts the MFMAs first and the rest behind.)
+        v4i ka[4], p[4][PT];
+#pragma unroll
+        for (int f = 0; f < 4; f++) ka[f] = kfrag(f);
+        s2[0] = s2[1] = (v16f){};
+#pragma unroll
+        for (int f = 0; f < NK; f++) {
+          s2[f & 1] = mfma_bf16(ka[f & 3], q[f >> 1], s2[f & 1]);
+          if (f + 4 < NK) ka[f & 3] = kfrag(f + 4);
+#pragma unroll
+          for (int g = f * 16 / NK; g < (f + 1) * 16 / NK; g++) {
+            const int m = g >> 2, x = g & 3, i = 8 * (m & 1) + 2 * x;
+            float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m >> 1][i], c, mcn));
+            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[m >> 1][i + 1], c, mcn));
+            l += p0;
+            l += p1;
+#pragma unroll
+            for (int y = 0; y < PT; y++) {
+              const uint32_t w = pack_bf16(p0, p1);
+              p[m][y][x] = (int)w;
+              p0 -= __uint_as_float(w << 16);
+              p1 -= __uint_as_float(w & 0xffff0000u);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+
+        // ---- O^T += V^T P^T, and between its MFMAs the widening
+        v4i va[4];
+        hide_v(key0 + BK);
+        pin();
+#pragma unroll
+        for (int f = 0; f < 4; f++) va[f] = vfrag(f);
+#pragma unroll
+        for (int f = 0; f < NV; f++) {
+#pragma unroll
+          for (int y = 0; y < PT; y++) o[f % ND] = mfma_bf16(va[f & 3], p[f / ND][y], o[f % ND]);
+          if (f + 4 < NV) va[f & 3] = vfrag(f + 4);
+          constexpr int PER = NV / (8 * TW);   // steps per piece
+          if (f % PER == 0) {
+            const int u = f / PER, v = u >> 3;
+            if (u & 4)
+              stage_v(v, u & 3);
+            else
+              stage_k(v, u & 3);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        load_k(at_or_none(key0 + 3 * BK));
+        load_v(at_or_none(key0 + 2 * BK));
+        kat ^= BUF;
+        vat ^= BUF;
+        kst ^= BUF;
+        vst ^= BUF;
+        __syncthreads();
+      };
+      for (int key0 = kbeg;; key0 += BK) {
+        block(key0, s, t);
+        key0 += BK;
+        if (key0 >= kend) break;
+        block(key0, t, s);
+        if (key0 + BK >= kend) break;
+      }
+
+      // ---- out: lane (n, h) holds 4 consecutive d of row n in each group of four registers
+      const bool whole = nj == nblk;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
+      const float ls = pair_sum(l);
+      if (valid) {
+        const float inv = !whole ? 1.0f : ls != 0.0f ? 1.0f / ls : 0.0f;   // no visible key: 0
+        const int64_t pr = slot * a.tile_rows + (row - row0);
+#pragma unroll
+        for (int j = 0; j < ND; j++)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            const int d = 32 * j + 2 * i + 4 * h;
+            const float4 x = make_float4(o[j][i] * inv, o[j][i + 1] * inv, o[j][i + 2] * inv, o[j][i + 3] * inv);
+            if (!whole)
+              *reinterpret_cast<float4*>(a.part_o + pr * D + d) = x;
+            else
+              kv4_store4(a, b, kvh, row, d, x);
+          }
+        if (!whole && h == 0) reinterpret_cast<float2*>(a.part_ml)[pr] = make_float2(mc, ls);
+      }
+    }
+    u0 += take;
+    if (u0 >= u1) return;
+    first = false;
+    in += take;
+    if (in == room * a.Hkv) {
+      in = 0;
+      gt++;
+    }
+  }
+}
+
+#define MXFA_KV4_TILED(D, SC, PT, OCC, NAME) \
+  extern "C" __global__ void __launch_bounds__(256, OCC) NAME(Kv4AttnArgs a) { kv4_tiled_impl<D, SC, PT>(a); }
+#define MXFA_KV4_TILED_ALL(D, OCC)                                          \
+  MXFA_KV4_TILED(D, false, 1, OCC, mxfa_kv4_tiled_d##D)               \
+  MXFA_KV4_TILED(D, true, 1, OCC, mxfa_kv4_tiled_d##D##_softcap)      \
+  MXFA_KV4_TILED(D, false, 3, OCC, mxfa_kv4_tiled_d##D##_f32)         \
+  MXFA_KV4_TILED(D, true, 3, OCC, mxfa_kv4_tiled_d##D##_softcap_f32)
+MXFA_KV4_TILED_ALL(64, 2)
+MXFA_KV4_TILED_ALL(128, 2)
+MXFA_KV4_TILED_ALL(256, 1)
+
+// The merge of the pieces of an item that several workgroups hold: O = sum O_p 2^(m_p - M) / sum l_p 2^(m_p -
+// M); 0 where nothing was visible.  A workgroup takes merge_rows rows of an item, D / 4 lanes of 4 d for each
+// of 256 / (D / 4) / merge_rows groups that take a row's pieces in turn: one row after the streaming form, whose
+// few rows may have a piece in every workgroup, as many as there are lanes for after the tiled one.
 extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_combine(Kv4AttnArgs a) {
-  __shared__ __attribute__((aligned(16))) float so[3][256];
-  __shared__ float sl[3];
-  const int D = blockDim.x, lanes = D / 4, grp = threadIdx.x / lanes, x = threadIdx.x % lanes;
-  const int bk = blockIdx.x / a.rows, r = blockIdx.x % a.rows;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + (int64_t)blockIdx.x * a.n_parts;
-  const float* po = a.part_o + (int64_t)blockIdx.x * a.n_parts * D + 4 * x;
-  float M = -INFINITY;
-  for (int p = 0; p < a.n_parts; p++) M = fmaxf(M, ml[p].x);
-  const float m0 = M == -INFINITY ? 0.0f : M;
-  float L = 0.0f;
+  __shared__ __attribute__((aligned(16))) float so[256 * 4];
+  __shared__ float sl[16];
+  const int D = a.D, lanes = D / 4, tid = threadIdx.x, x = tid % lanes, ngrp = 256 / lanes / a.merge_rows;
+  const int grp = tid / lanes % ngrp, lane = tid & 63;
+  const int per = (min(a.tile_rows, a.rows) + a.merge_rows - 1) / a.merge_rows;
+  const int item = blockIdx.x / per, gt = item / a.Hkv, kvh = item % a.Hkv;
+  const int rr = blockIdx.x % per * a.merge_rows + tid / lanes / ngrp;   // row in the tile
+  int b, row0, i0, i1;
+  kv4_tile(a, gt, b, row0, i0, i1);
+  const int share = kv4_share(a, kv4_line(a, lane, a.B * a.n_rt));
+  const int nblk = kv4_blocks(a, gt), start = kv4_line(a, lane, gt) + kvh * kv4_room(nblk);
+  const int w0 = start / share, np = (start + nblk - 1) / share - w0 + 1;
+  if (np == 1) return;                     // (written by its workgroup)
+  const int r = row0 + rr;
+  const bool have = rr < a.tile_rows && r < a.rows;
+  // piece p lies in slot 2 (w0 + p); the first one in 2 w0 + 1 where its workgroup's share begins before it
+  const int odd = start % share ? 1 : 0;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
+  auto at = [&](int p) { return (int64_t)(2 * (w0 + p) + (p == 0 ? odd : 0)) * a.tile_rows + rr; };
+  float M = -INFINITY, L = 0.0f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = grp; p < a.n_parts; p += 4) {
-    const float w = __builtin_amdgcn_exp2f(ml[p].x - m0);
-    L += ml[p].y * w;
-    const float4 o = *reinterpret_cast<const float4*>(po + (int64_t)p * D);
-    acc.x += o.x * w; acc.y += o.y * w; acc.z += o.z * w; acc.w += o.w * w;
+  if (have) {
+#pragma unroll 4
+    for (int p = 0; p < np; p++) M = fmaxf(M, ml[at(p)].x);
+    const float m0 = M == -INFINITY ? 0.0f : M;
+#pragma unroll 4
+    for (int p = grp; p < np; p += ngrp) {
+      const float2 v = ml[at(p)];
+      const float4 o = *reinterpret_cast<const float4*>(a.part_o + at(p) * D + 4 * x);
+      const float w = __builtin_amdgcn_exp2f(v.x - m0);
+      L += v.y * w;
+      acc.x += o.x * w; acc.y += o.y * w; acc.z += o.z * w; acc.w += o.w * w;
+    }
   }
-  if (grp) {
-    *reinterpret_cast<float4*>(&so[grp - 1][4 * x]) = acc;
-    if (x == 0) sl[grp - 1] = L;
+  if (ngrp > 1) {
+    *reinterpret_cast<float4*>(&so[4 * tid]) = acc;
+    if (x == 0) sl[tid / lanes] = L;
+    __syncthreads();
+    if (grp) return;
+    for (int i = 1; i < ngrp; i++) {
+      const float4 o = *reinterpret_cast<const float4*>(&so[4 * (tid + i * lanes)]);
+      acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+      L += sl[tid / lanes + i];
+    }
   }
-  __syncthreads();
-  if (grp) return;
-  for (int i = 0; i < 3; i++) {
-    const float4 o = *reinterpret_cast<const float4*>(&so[i][4 * x]);
-    acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
-    L += sl[i];
-  }
+  if (!have) return;
   const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-  acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
-  const int b = bk / a.Hkv, kvh = bk % a.Hkv;
-  const int64_t oo = b * a.o_b + (kvh * a.group + r % a.group) * a.o_h + r / a.group * a.o_t + 4 * x;
-  if (a.o_bf16)
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + oo) = make_uint2(pack_bf16(acc.x, acc.y), pack_bf16(acc.z, acc.w));
-  else
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.o) + oo) = acc;
+  kv4_store4(a, b, kvh, r, 4 * x, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
 }

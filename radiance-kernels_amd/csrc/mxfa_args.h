@@ -80,13 +80,16 @@ struct Kv4AttnArgs {
   const uint8_t* vs;
   const int* kv_len;  // keys of each sequence [B], or NULL: Sk
   uint8_t* o;         // bf16 or fp32
-  float* part_o;      // [B * Hkv * rows][n_parts][D], unnormalized
-  float* part_ml;     // [B * Hkv * rows][n_parts][2]: the reference exponent (log2 units) and the row sum
+  float* part_o;      // [2 n_wg slots][tile_rows][D], unnormalized
+  float* part_ml;     // [2 n_wg slots][tile_rows][2]: the reference exponent (log2 units) and the row sum
   int64_t q_b, q_h, q_t, o_b, o_h, o_t;   // element strides
   int B, Hq, Hkv, Sq, Sk, L;
   int group, rows;    // Hq / Hkv; rows of a KV head: group * Sq, row r = query r / group of head r % group
   int q_pos0, window, causal, o_bf16;
-  int n_rt, n_parts;  // row tiles of a KV head; parts of the key range
+  int D, n_rt, tile_rows;   // row tiles of a KV head and their rows
+  int n_wg;           // workgroups that share the blocks of all items; 0: one workgroup per item
+  int min_share;      // blocks of a workgroup's share at least
+  int merge_rows;     // rows of a workgroup of the merge
   float c_log2, sc_u, cap_log2;
 };
 

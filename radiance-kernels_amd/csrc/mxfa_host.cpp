@@ -84,8 +84,9 @@ const char* const kKernelNames[] = {
     MXFA_DECODE_BLK_NAMES(64), MXFA_DECODE_BLK_NAMES(128), MXFA_DECODE_BLK_NAMES(256),
     "mxfa_kv4_append_f32", "mxfa_kv4_append_bf16", "mxfa_kv4_read_f32", "mxfa_kv4_read_bf16", "mxfa_kv4_combine",
     "mxfa_rmsnorm_quant_f32", "mxfa_rmsnorm_quant_bf16",
+#define MXFA_KV4_NAMES4(P) P, P "_softcap", P "_f32", P "_softcap_f32"
 #define MXFA_KV4_NAMES(D) \
-  "mxfa_kv4_attn_d" #D, "mxfa_kv4_attn_d" #D "_softcap", "mxfa_kv4_attn_d" #D "_f32", "mxfa_kv4_attn_d" #D "_softcap_f32"
+  MXFA_KV4_NAMES4("mxfa_kv4_attn_d" #D "_t1"), MXFA_KV4_NAMES4("mxfa_kv4_attn_d" #D "_t2"), MXFA_KV4_NAMES4("mxfa_kv4_tiled_d" #D)
     MXFA_KV4_NAMES(64), MXFA_KV4_NAMES(128), MXFA_KV4_NAMES(256),
 };
 constexpr int kNumKernels = sizeof(kKernelNames) / sizeof(kKernelNames[0]);
@@ -1025,24 +1026,33 @@ mxfa_status check_kv4_attn(const mxfa_kv4_attn_params* p) {
   return MXFA_OK;
 }
 
-// How a call is dealt to workgroups.
+// How a call is dealt to workgroups: the streaming form (one tile of at most 32 rows) or the tiled one, and one
+// workgroup per item or equal shares of the line of all items' blocks (kv4_my_share in k_kv4.hip).
 struct Kv4Plan {
-  int n_rt, n_parts;       // row tiles of a KV head; parts of the key range
-  int64_t items;           // workgroups
+  bool tiled;
+  int n_rt, tile_rows, n_wg, min_share;
+  int64_t items;           // (sequence, row tile, KV head)
   size_t ws;
 };
 
 mxfa_status kv4_plan(const mxfa_kv4_attn_params* p, Kv4Plan* out) {
   const int64_t rows = (int64_t)(p->num_q_heads / p->num_kv_heads) * p->seq_q;
-  const int64_t bk = (int64_t)p->batch * p->num_kv_heads;
-  out->n_rt = (int)((rows + 15) / 16);
-  if (bk > (int64_t)UINT32_MAX / 256 / out->n_rt)
-    return fail(MXFA_ERR_UNSUPPORTED, "the call needs more than 2^32 work-items in one launch: split it");
-  const int64_t tiles = bk * out->n_rt, blocks = (p->seq_k + 63) / 64;
-  int64_t n = std::min<int64_t>((512 + tiles - 1) / tiles, (blocks + 3) / 4);
-  out->n_parts = (int)std::max<int64_t>(n, 1);
-  out->items = tiles * out->n_parts;
-  out->ws = out->n_parts > 1 ? (size_t)bk * rows * out->n_parts * (p->head_dim + 2) * sizeof(float) : 0;
+  const int64_t bk = (int64_t)p->batch * p->num_kv_heads, blocks = (p->seq_k + 63) / 64;
+  out->tiled = rows > 32;
+  out->tile_rows = out->tiled ? 128 : rows <= 16 ? 16 : 32;
+  out->n_rt = (int)((rows + out->tile_rows - 1) / out->tile_rows);
+  // (the device numbers blocks with 32 bits)
+  if (bk > (int64_t)INT32_MAX / 256 / out->n_rt || bk * out->n_rt > (int64_t)INT32_MAX / (blocks + 8))
+    return fail(MXFA_ERR_UNSUPPORTED, "the call walks more than 2^31 blocks of keys: split it");
+  out->items = bk * out->n_rt;
+  // One workgroup per item for short caches, where a share would be a piece too small to pay for its merge, and for so
+  // many items that their different lengths even out; else as many shares as workgroups fit the chip at once: two
+  // per CU, at D = 256 with more than 16 rows one.
+  out->min_share = 8;
+  const int slots = p->head_dim == 256 && rows > 16 ? 256 : 512;
+  const bool per_item = blocks <= 2 * out->min_share || out->items >= 8 * slots;
+  out->n_wg = per_item ? 0 : slots;
+  out->ws = per_item ? 0 : (size_t)2 * out->n_wg * out->tile_rows * (p->head_dim + 2) * sizeof(float);
   return MXFA_OK;
 }
 
@@ -1065,11 +1075,11 @@ mxfa_status mxfa_kv4_read(const mxfa_kv4_shape* c, int32_t x_fmt, const uint8_t*
                   stream);
 }
 
-mxfa_status mxfa_kv4_attention_plan(const mxfa_kv4_attn_params* p, int32_t* n_parts, size_t* workspace_bytes) {
+mxfa_status mxfa_kv4_attention_plan(const mxfa_kv4_attn_params* p, int32_t* n_shares, size_t* workspace_bytes) {
   if (mxfa_status st = check_kv4_attn(p)) return st;
   Kv4Plan plan;
   if (mxfa_status st = kv4_plan(p, &plan)) return st;
-  if (n_parts) *n_parts = plan.n_parts;
+  if (n_shares) *n_shares = plan.n_wg;
   if (workspace_bytes) *workspace_bytes = plan.ws;
   return MXFA_OK;
 }
@@ -1102,28 +1112,30 @@ mxfa_status mxfa_kv4_attention(const mxfa_kv4_attn_params* p, const void* q, con
   a.window = p->window < (1 << 30) ? p->window : 0;              // (positions stay below 2^30: no key is that far behind)
   a.causal = p->causal != 0;
   a.o_bf16 = bf16;
-  a.n_rt = plan.n_rt; a.n_parts = plan.n_parts;
+  a.D = p->head_dim; a.n_rt = plan.n_rt; a.tile_rows = plan.tile_rows; a.n_wg = plan.n_wg; a.min_share = plan.min_share;
+  a.merge_rows = plan.tiled ? 1024 / p->head_dim : 1;
   const float log2e = 1.4426950408889634f;
   a.c_log2 = p->softmax_scale * log2e;
   if (p->softcap > 0.0f) {
     a.sc_u = p->softmax_scale / p->softcap;
     a.cap_log2 = p->softcap * log2e;
   }
-  const int64_t rows = (int64_t)p->batch * p->num_kv_heads * a.rows;
-  if (plan.n_parts > 1) {
+  if (plan.n_wg) {
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + rows * plan.n_parts * p->head_dim;
+    a.part_ml = a.part_o + (size_t)2 * plan.n_wg * plan.tile_rows * p->head_dim;
   }
-  if (mxfa_status st = check_grid(plan.items, 256)) return st;
-  if (mxfa_status st = check_grid(plan.n_parts > 1 ? rows : 0, p->head_dim)) return st;
+  const int64_t grid = plan.n_wg ? plan.n_wg : plan.items, merge = plan.n_wg ? plan.items * ((std::min(plan.tile_rows, a.rows) + a.merge_rows - 1) / a.merge_rows) : 0;
+  if (mxfa_status st = check_grid(grid, 256)) return st;
+  if (mxfa_status st = check_grid(merge, 256)) return st;
   DeviceModule* dm;
   if (mxfa_status st = module_for_current(&dm)) return st;
   char name[48];
-  std::snprintf(name, sizeof name, "mxfa_kv4_attn_d%d%s%s", p->head_dim, p->softcap > 0.0f ? "_softcap" : "", bf16 ? "" : "_f32");
+  std::snprintf(name, sizeof name, "mxfa_kv4_%s_d%d%s%s%s", plan.tiled ? "tiled" : "attn", p->head_dim,
+                plan.tiled ? "" : plan.tile_rows == 16 ? "_t1" : "_t2", p->softcap > 0.0f ? "_softcap" : "", bf16 ? "" : "_f32");
   void* args[] = {&a};
-  if (mxfa_status st = launch(dm, name, dim3((unsigned)plan.items), dim3(256), args, stream)) return st;
-  if (plan.n_parts == 1) return MXFA_OK;
-  return launch(dm, "mxfa_kv4_combine", dim3((unsigned)rows), dim3((unsigned)p->head_dim), args, stream);
+  if (mxfa_status st = launch(dm, name, dim3((unsigned)grid), dim3(256), args, stream)) return st;
+  if (!plan.n_wg) return MXFA_OK;
+  return launch(dm, "mxfa_kv4_combine", dim3((unsigned)merge), dim3(256), args, stream);
 }
 
 mxfa_status mxfa_rmsnorm_quantize(const mxfa_norm_params* p, const void* x, const void* residual, const void* weight, void* h,

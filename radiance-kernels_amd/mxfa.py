@@ -591,7 +591,7 @@ def make_kv4_params(B, Hq, Hkv, Sq, Sk, D, max_len, causal=True, q_pos0=0, windo
 
 
 def kv4_attention_plan(p):
-    """(parts of the key range, workspace bytes) of kv4_attention for p; without parts the bytes are 0."""
+    """(shares of the key blocks, workspace bytes) of kv4_attention for p; without shares the bytes are 0."""
     n, ws = ctypes.c_int32(0), ctypes.c_size_t(0)
     _check(lib().mxfa_kv4_attention_plan(p, ctypes.byref(n), ctypes.byref(ws)))
     return n.value, ws.value

@@ -108,15 +108,16 @@ def attention(q, K, V, lens, causal=True, q_pos0=None, window=0, scale=None, sof
     return O, A, X, Y
 
 
-def attention_bound(O, A, X, Y, D, keys, f32, softcap=0.0):
+def attention_bound(O, A, X, Y, D, keys, f32, rows, softcap=0.0):
     """How far a kernel's O may be, element by element.  With u = 2^-24: a score is a sum of D exact products added
     in fp32, off by at most D u Y; scaling, the reference exponent and the difference round three times at
     u max(X, 1) each, twice that range; tanh by exponentials is off by some 8 u of its cap.  P is then off by ln 2
-    times that, by two steps of exp2 and by the terms that enter the product (2^-17 for two, 2^-25 for three), O
+    times that, by two steps of exp2 and by what its bf16 terms leave of it (2^-8 for each: three terms for fp32 O, for
+    bf16 O two up to 32 rows of a KV head and one beyond), O
     by twice P's relative error of A (numerator and sum) and by `keys` roundings in each sum; then O is rounded."""
     u = 2.0 ** -24
     x = u * (D * Y + 6 * max(X, 1.0) + 8 * softcap * math.log2(math.e))
-    p = math.log(2) * x + 4 * u + (2.0 ** -25 if f32 else 2.0 ** -17)
+    p = math.log(2) * x + 4 * u + 2.0 ** -(8 * (3 if f32 else 2 if rows <= 32 else 1))
     return 2 * (p + (keys + 16) * u) * A + (u if f32 else 2.0 ** -8) * O.abs() + keys * 2.0 ** -126
 
 

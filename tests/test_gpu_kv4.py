@@ -208,7 +208,7 @@ def _check(got, want, p, keys, what=""):
     O, A, X, Y = want
     f32 = p.o_fmt == mxfa.C_F32
     assert got.dtype == (torch.float32 if f32 else torch.bfloat16)
-    bound = R.attention_bound(O, A, X, Y, p.head_dim, keys, f32, p.softcap)
+    bound = R.attention_bound(O, A, X, Y, p.head_dim, keys, f32, p.num_q_heads // p.num_kv_heads * p.seq_q, p.softcap)
     err = (got.double().cpu() - O).abs()
     worst = float((err / bound).max())
     rel = float((got.double().cpu() - O).norm() / max(float(O.norm()), 1e-30))
@@ -283,11 +283,11 @@ def test_attention_split_over_a_long_cache(B, Hq, Hkv, Sq, D, n, kw, f32):
     lens = [n] if B == 1 else [n, 40]
     q, cache, lt = _problem(B, Hq, Hkv, Sq, D, L, lens, seed=n + Sq, amp=1.5)
     p = mxfa.make_kv4_params(B, Hq, Hkv, Sq, n, D, L, o_fmt=mxfa.C_F32 if f32 else mxfa.C_BF16, **kw)
-    parts, ws = mxfa.kv4_attention_plan(p)
-    assert parts > 1
+    shares, ws = mxfa.kv4_attention_plan(p)
+    assert shares > 1
     # a workspace of garbage, larger than needed
     got = mxfa.kv4_attention(p, q, cache, kv_len=lt, workspace=torch.full((ws + 512,), 255, dtype=torch.uint8, device=DEV))
-    _check(got, _want(q, cache, lens, p, False), p, n, f"{parts} parts")
+    _check(got, _want(q, cache, lens, p, False), p, n, f"{shares} shares")
 
 
 def test_attention_lengths_are_clamped():
@@ -332,7 +332,7 @@ def test_attention_of_extreme_scores(Sq, amp):
         got = mxfa.kv4_attention(p, q, cache, kv_len=lt)
         O, A, X, Y = _want(q, cache, [n], p, False)
         assert X > 10 * amp
-        bound = R.attention_bound(O, A, X, Y, D, n, f32)
+        bound = R.attention_bound(O, A, X, Y, D, n, f32, Hq // Hkv * Sq)
         err = (got.double().cpu() - O).abs()
         assert bool((err <= bound).all()), float((err / bound).max())
 
@@ -436,8 +436,8 @@ def test_graph_and_streams():
     g = torch.Generator(device=DEV).manual_seed(72)
     rows = torch.randn((steps, B, 1, Hq + 2 * Hkv, D), generator=g, device=DEV).bfloat16()
     p = mxfa.make_kv4_params(B, Hq, Hkv, 1, L, D, L)
-    parts, ws_bytes = mxfa.kv4_attention_plan(p)
-    assert parts > 1
+    shares, ws_bytes = mxfa.kv4_attention_plan(p)
+    assert shares > 1
 
     def make():
         c = mxfa.Kv4Cache.of(cache.k.clone(), cache.ks.clone(), cache.v.clone(), cache.vs.clone())

@@ -89,15 +89,15 @@ def test_attention_pointers_strides_and_workspace():
     assert _attend(p, os_=S(8, 4, 8)) == 1 and "o strides" in _err()
     assert _attend(_params(o_fmt=0), os_=S(8, 2, 8)) == 1
     long = _params(B=1, Sk=100000, max_len=100000)
-    parts, need = mxfa.kv4_attention_plan(long)
-    assert parts > 1 and need >= 8 * parts * (128 + 2) * 4
+    shares, need = mxfa.kv4_attention_plan(long)
+    assert shares > 1 and need >= 2 * 4 * shares * (128 + 2) * 4
     assert _attend(long, ws=None) == 5 and _attend(long, ws_bytes=need - 1) == 5 and "workspace needs" in _err()
     assert _attend(long, ws=FAKE + 8) == 1
 
 
-def test_plan_without_parts_needs_no_workspace():
-    for kw in (dict(), dict(B=600), dict(Sq=4000, Sk=4000, max_len=4000)):
-        assert mxfa.kv4_attention_plan(_params(**kw)) == (1, 0), kw
+def test_plan_of_short_caches_and_large_batches_needs_no_workspace():
+    for kw in (dict(), dict(B=600), dict(Sq=900, Sk=900, max_len=1024), dict(B=2048, Sk=8192, max_len=8192)):
+        assert mxfa.kv4_attention_plan(_params(**kw)) == (0, 0), kw
 
 
 def _norm(rows=4, cols=256, fmt=mxfa.C_BF16, eps=1e-6, off=0.0, ld=0, x=FAKE, res=None, w=FAKE, h=None, codes=FAKE, sc=FAKE):
