@@ -201,9 +201,15 @@ __device__ __forceinline__ float col_max(float x) {
 struct Kv4Seq {
   int len, pos0;
 };
+// UNIFORM: b is the same in all lanes (the length then lives in scalar registers, also where stores lie between).
+template <bool UNIFORM>
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b) {
   Kv4Seq s;
-  s.len = a.kv_len ? min(max(a.kv_len[b], 0), a.Sk) : a.Sk;
+  s.len = a.Sk;
+  if (a.kv_len) {
+    const int len = a.kv_len[b];
+    s.len = min(max(UNIFORM ? __builtin_amdgcn_readfirstlane(len) : len, 0), a.Sk);
+  }
   s.pos0 = a.kv_len ? s.len - a.Sq : a.q_pos0;
   return s;
 }
@@ -221,10 +227,11 @@ __device__ __forceinline__ void kv4_tile(const Kv4AttnArgs& a, int gt, int& b, i
   i0 = a.n_rt == 1 ? 0 : row0 / a.group;
   i1 = a.n_rt == 1 ? a.Sq - 1 : (min(row0 + a.tile_rows, a.rows) - 1) / a.group;
 }
+template <bool UNIFORM>
 __device__ __forceinline__ int kv4_blocks(const Kv4AttnArgs& a, int gt) {
   int b, row0, i0, i1, lo, hi, t;
   kv4_tile(a, gt, b, row0, i0, i1);
-  const Kv4Seq s = kv4_seq(a, b);
+  const Kv4Seq s = kv4_seq<UNIFORM>(a, b);
   kv4_limits(a, s, i0, lo, t);
   kv4_limits(a, s, i1, t, hi);
   return hi >= lo ? hi / KV4_BK - lo / KV4_BK + 1 : 1;
@@ -233,65 +240,94 @@ __device__ __forceinline__ int kv4_blocks(const Kv4AttnArgs& a, int gt) {
 // (Q, the first loads, the merge: some 8 blocks' worth), so that a share does not hold many of them.
 __device__ __forceinline__ int kv4_room(int nblk) { return nblk < 32 ? nblk + 8 : nblk; }
 
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) x += __shfl_xor(x, k);
+// Inclusive prefix sum over a wave, by DPP (shifts inside rows of 16, then the row totals broadcast on).
+__device__ __forceinline__ int wave_prefix(int x) {
+  auto add = [&](auto ctrl, auto rows) { x += __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false); };
+  add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});   // row_shr:1
+  add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});   // row_shr:2
+  add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});   // row_shr:4
+  add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});   // row_shr:8
+  add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});   // row_bcast:15 to rows 1 and 3
+  add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});   // row_bcast:31 to rows 2 and 3
   return x;
 }
-// Share of a workgroup for a line of `total`.
-__device__ __forceinline__ int kv4_share(const Kv4AttnArgs& a, int total) {
-  const int s = (total + a.n_wg - 1) / a.n_wg;
-  return max((s + KV4_NW - 1) / KV4_NW * KV4_NW, a.min_share);
-}
-// Room of the items of row tiles before g_end.
-__device__ __forceinline__ int kv4_line(const Kv4AttnArgs& a, int lane, int g_end) {
-  int n = 0;
-  for (int gt = lane; gt < g_end; gt += 64) n += kv4_room(kv4_blocks(a, gt));
-  return __builtin_amdgcn_readfirstlane(wave_sum(n)) * a.Hkv;
+// How the blocks are dealt.  With few items (a.cut: at most half as many as workgroups), each is cut into pieces of equal
+// size, a multiple of the waves, and every piece is a workgroup of its own: `share` is the smallest size (to a
+// sixteenth) with which there are workgroups for all pieces.  With more items the line of all of them is cut into
+// equal shares, each a workgroup that walks the pieces in it.  (16 sequences of 375 to 6,001 tokens, 20 rows of
+// 8 KV heads: 34.0 us from a line, whose workgroups with two pieces take 24 and those with one 15; cut 30.9.)
+__device__ __forceinline__ uint32_t kv4_pieces(uint32_t nblk, uint32_t share) { return (nblk + share - 1) / share; }
+__device__ __forceinline__ uint32_t kv4_up(uint32_t n) { return (n + KV4_NW - 1) / KV4_NW * KV4_NW; }
+// nblk0: kv4_blocks of tile `lane` (0 past the last).
+__device__ __forceinline__ uint32_t kv4_share(const Kv4AttnArgs& a, int lane, uint32_t nblk0) {
+  const int groups = a.B * a.n_rt;
+  auto sum = [&](auto f) {
+    uint32_t n = nblk0 ? f(nblk0) : 0;
+    for (int gt = 64 + lane; gt < groups; gt += 64) n += f(kv4_blocks<false>(a, gt));
+    return __builtin_amdgcn_readlane(wave_prefix(n), 63) * (uint32_t)a.Hkv;
+  };
+  const uint32_t total = sum([&](uint32_t n) { return a.cut ? n : kv4_room(n); });
+  uint32_t s = max(kv4_up((total + a.n_wg - 1) >> a.wg_log2), (uint32_t)a.min_share);
+  if (a.cut) {
+    const uint32_t step = kv4_up(s >> 4);
+    while (sum([&](uint32_t n) { return kv4_pieces(n, s); }) > (uint32_t)a.n_wg) s += step;
+  }
+  return s;
 }
 
-// Places u0 .. u1 - 1 of the line are this workgroup's: row tile gt, `in` into its items.  False: none.
-__device__ __forceinline__ bool kv4_my_share(const Kv4AttnArgs& a, int lane, int& u0, int& u1, int& gt, int& in) {
+// This workgroup's part of the line: `left` places from j0 of item (row tile gt, KV head kvh) on; an item's later pieces
+// hold `share`.  False: none.
+struct Kv4Part {
+  int gt, kvh, j0, left, share;
+};
+__device__ __forceinline__ bool kv4_my_part(const Kv4AttnArgs& a, int lane, Kv4Part& w) {
   if (!a.n_wg) {                           // one workgroup per item, the tiles that see most keys first
-    gt = a.B * a.n_rt - 1 - blockIdx.x / a.Hkv;
-    u0 = 0;
-    u1 = kv4_room(kv4_blocks(a, gt));
-    in = blockIdx.x % a.Hkv * u1;
+    w.gt = a.B * a.n_rt - 1 - blockIdx.x / a.Hkv;
+    w.kvh = blockIdx.x % a.Hkv;
+    w.j0 = 0;
+    w.left = w.share = kv4_room(kv4_blocks<true>(a, w.gt));
     return true;
   }
   const int groups = a.B * a.n_rt;
-  int mine = lane < groups ? kv4_room(kv4_blocks(a, lane)) * a.Hkv : 0, sum = mine;
-  auto prefix = [&] {                      // inclusive
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-      const int x = __shfl_up(sum, k);
-      sum += lane >= k ? x : 0;
-    }
-  };
-  prefix();
-  const int total = groups <= 64 ? __builtin_amdgcn_readlane(sum, 63) : kv4_line(a, lane, groups);
-  const int share = kv4_share(a, total);
-  u0 = blockIdx.x * share;
-  if (u0 >= total) return false;
-  u1 = min(total, u0 + share);
-  for (int g0 = 0, at = 0;;) {             // at: places before tile g0
+  uint32_t nblk = lane < groups ? kv4_blocks<false>(a, lane) : 0;
+  const uint32_t share = kv4_share(a, lane, nblk), u0 = a.cut ? blockIdx.x : blockIdx.x * share;
+  uint32_t at = 0;                         // places (cut: pieces) before tile g0
+  for (int g0 = 0; g0 < groups; g0 += 64) {
+    if (g0) nblk = g0 + lane < groups ? kv4_blocks<false>(a, g0 + lane) : 0;
+    const uint32_t each = !nblk ? 0 : a.cut ? kv4_pieces(nblk, share) : kv4_room(nblk), mine = each * a.Hkv;
+    const uint32_t sum = wave_prefix(mine);
     const uint64_t past = __ballot(at + sum > u0);
     if (past) {
       const int l = __builtin_ctzll(past);
-      gt = g0 + l;
-      in = u0 - (at + __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
+      const uint32_t n = __builtin_amdgcn_readlane(nblk, l), per = __builtin_amdgcn_readlane(each, l);
+      const uint32_t in = u0 - (at + __builtin_amdgcn_readlane(sum, l) - per * a.Hkv);
+      w.gt = g0 + l;
+      w.kvh = in / per;
+      w.j0 = in - w.kvh * per;
+      w.left = w.share = share;            // (the walk ends at the last tile)
+      if (a.cut) {
+        const uint32_t size = kv4_up((n + per - 1) / per);
+        w.j0 *= size;
+        w.share = size;
+        w.left = min((int)size, (int)n - w.j0);
+        return w.left > 0;
+      }
       return true;
     }
     at += __builtin_amdgcn_readlane(sum, 63);
-    g0 += 64;
-    sum = mine = g0 + lane < groups ? kv4_room(kv4_blocks(a, g0 + lane)) * a.Hkv : 0;
-    prefix();
   }
+  return false;
+}
+// The first piece of an item (nj of its nblk blocks) leaves in the workspace where the item's pieces lie: its own slot
+// and their number.  The second lies in slot `a.cut ? w + 1 : 2 (w + 1)` for workgroup w.
+__device__ __forceinline__ void kv4_note_item(const Kv4AttnArgs& a, const Kv4Part& w, int nblk, int nj, int slot) {
+  if (a.n_wg && w.j0 == 0 && threadIdx.x == 0)
+    reinterpret_cast<int2*>(a.pieces)[w.gt * a.Hkv + w.kvh] = make_int2(slot, 1 + (uint32_t)(nblk - nj + w.share - 1) / (uint32_t)w.share);
 }
 
-// Row r of a KV head's O: 4 values from d on, or (a piece of an item) to the workspace.
-__device__ __forceinline__ void kv4_store4(const Kv4AttnArgs& a, int b, int kvh, int r, int d, float4 x) {
-  const int64_t o = b * a.o_b + (kvh * a.group + r % a.group) * a.o_h + r / a.group * a.o_t + d;
+// 4 values of O (query i, head hd) from d on.
+__device__ __forceinline__ void kv4_store4(const Kv4AttnArgs& a, int b, int hd, int i, int d, float4 x) {
+  const int64_t o = b * a.o_b + hd * a.o_h + i * a.o_t + d;
   if (a.o_bf16)
     *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.o) + o) = make_uint2(pack_bf16(x.x, x.y), pack_bf16(x.z, x.w));
   else
@@ -312,16 +348,18 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
 
-  int u0, u1, gt, in;
-  if (!kv4_my_share(a, lane, u0, u1, gt, in)) return;
+  Kv4Part w;
+  if (!kv4_my_part(a, lane, w)) return;
+  const bool young = (int)blockIdx.x >= 256;   // (the first 256 workgroups take a CU each)
   bool first = true;
 
   while (true) {
-    const int nblk = kv4_blocks(a, gt), room = kv4_room(nblk), b = gt;       // (one row tile)
-    const int kvh = in / room, j0 = in - kvh * room, take = min(room - j0, u1 - u0), nj = min(nblk - j0, take);
+    const int nblk = kv4_blocks<true>(a, w.gt), b = w.gt, kvh = w.kvh, j0 = w.j0;       // (one row tile)
+    const int take = min(kv4_room(nblk) - j0, w.left), nj = min(nblk - j0, take);
     if (nj > 0) {
+    const int slot = a.cut ? blockIdx.x : 2 * blockIdx.x + (first ? 0 : 1);
     const int bk = b * a.Hkv + kvh;
-    const Kv4Seq seq = kv4_seq(a, b);
+    const Kv4Seq seq = kv4_seq<true>(a, b);
     // each column's keys, and those that every column sees or any does
     int klo[NT], khi[NT], klo_all, khi_all, klo_any, khi_any;
     kv4_limits(a, seq, 0, klo_any, khi_all);
@@ -332,7 +370,7 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
     for (int t = 0; t < NT; t++) {
       const int row = 16 * t + n;
       const bool valid = row < a.rows;
-      const int qi = valid ? row / a.group : 0, hd = kvh * a.group + (valid ? row % a.group : 0);
+      const int qi = valid ? row * a.group_inv >> 16 : 0, hd = kvh * a.group + (valid ? row - qi * a.group : 0);
       kv4_limits(a, seq, qi, klo[t], khi[t]);
       const uint16_t* qp = reinterpret_cast<const uint16_t*>(a.q) + b * a.q_b + hd * a.q_h + qi * a.q_t;
 #pragma unroll
@@ -417,6 +455,15 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
     load_v(kfirst < kend ? kfirst : a.L);
     __builtin_amdgcn_sched_barrier(0);
     for (int key0 = kfirst; key0 < kend; key0 += NW * BK) {
+      // Of two workgroups on a CU the older one's waves are served first and end well before the younger one's, which
+      // then has the CU to itself, too few waves to fill it: three blocks of four the younger has priority (64 x 8,192
+      // tokens: 94.4 us without, 92.1 so).
+      if (young) {
+        if (((key0 - kfirst) / (NW * BK) & 3) == 3)
+          __builtin_amdgcn_s_setprio(0);
+        else
+          __builtin_amdgcn_s_setprio(1);
+      }
       const int next = key0 + NW * BK < kend ? key0 + NW * BK : a.L;
       const bool masked = key0 < klo_all || key0 + BK - 1 > khi_all;
       // ---- S^T
@@ -547,7 +594,7 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
 
     // ---- merge the waves, a tile of columns at a time: d = (4 g + i) ND + j of column n
     const bool whole = nj == nblk;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
+    kv4_note_item(a, w, nblk, nj, slot);
 #pragma unroll
     for (int t = 0; t < NT; t++) {
       l[t] += __shfl_xor(l[t], 16);
@@ -567,6 +614,7 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
       // thread (col, x) = (tid / 16, tid % 16): 4 consecutive d at 4 x, 4 x + 64, ...
       const int col = tid >> 4, d0 = 4 * (tid & 15), r = 16 * t + col;
       if (r >= a.rows) continue;
+      const int qi = r * a.group_inv >> 16;
       float M = -INFINITY, Ls = 0.0f, wt[NW];
 #pragma unroll
       for (int w = 0; w < NW; w++) M = fmaxf(M, sml[w][col][0]);
@@ -586,20 +634,20 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
         }
         acc.x *= inv; acc.y *= inv; acc.z *= inv; acc.w *= inv;
         if (!whole)
-          *reinterpret_cast<float4*>(a.part_o + (slot * a.tile_rows + r) * D + d) = acc;
+          *reinterpret_cast<float4*>(a.part_o + ((int64_t)slot * a.tile_rows + r) * D + d) = acc;
         else
-          kv4_store4(a, b, kvh, r, d, acc);
+          kv4_store4(a, b, kvh * a.group + r - qi * a.group, qi, d, acc);
       }
-      if (!whole && d0 == 0) reinterpret_cast<float2*>(a.part_ml)[slot * a.tile_rows + r] = make_float2(M, Ls);
+      if (!whole && d0 == 0) reinterpret_cast<float2*>(a.part_ml)[(int64_t)slot * a.tile_rows + r] = make_float2(M, Ls);
     }
     }
-    u0 += take;
-    if (u0 >= u1) return;
+    w.left -= take;
+    if (w.left <= 0) return;
     first = false;
-    in += take;
-    if (in == room * a.Hkv) {
-      in = 0;
-      gt++;
+    w.j0 = 0;
+    if (++w.kvh == a.Hkv) {
+      w.kvh = 0;
+      if (++w.gt == a.B * a.n_rt) return;
     }
   }
 }
@@ -646,18 +694,20 @@ __device__ __forceinline__ void kv4_tiled_impl(const Kv4AttnArgs& a) {
   __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * BUF];   // K, K, V, V
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
-  int u0, u1, gt, in;
-  if (!kv4_my_share(a, lane, u0, u1, gt, in)) return;
+  Kv4Part w;
+  if (!kv4_my_part(a, lane, w)) return;
+  const bool young = (int)blockIdx.x >= 256;   // (the first 256 workgroups take a CU each)
   bool first = true;
 
   while (true) {
-    const int nblk = kv4_blocks(a, gt), room = kv4_room(nblk);
-    const int kvh = in / room, j0 = in - kvh * room, take = min(room - j0, u1 - u0), nj = min(nblk - j0, take);
+    const int nblk = kv4_blocks<true>(a, w.gt), kvh = w.kvh, j0 = w.j0;
+    const int take = min(kv4_room(nblk) - j0, w.left), nj = min(nblk - j0, take);
     if (nj > 0) {
+      const int slot = a.cut ? blockIdx.x : 2 * blockIdx.x + (first ? 0 : 1);
       int b, row0, i0, i1;
-      kv4_tile(a, gt, b, row0, i0, i1);
+      kv4_tile(a, w.gt, b, row0, i0, i1);
       const int bk = b * a.Hkv + kvh;
-      const Kv4Seq seq = kv4_seq(a, b);
+      const Kv4Seq seq = kv4_seq<true>(a, b);
       int klo_any, khi_any, t0, t1;
       kv4_limits(a, seq, i0, klo_any, t0);
       kv4_limits(a, seq, i1, t1, khi_any);
@@ -809,6 +859,12 @@ __device__ __forceinline__ void kv4_tiled_impl(const Kv4AttnArgs& a) {
       __syncthreads();
 
       auto block = [&](int key0, v16f(&s)[2], v16f(&s2)[2]) {
+        if (young) {                           // (as in the streaming form; 290.3 us without, 284.8 so)
+          if ((key0 / BK & 3) == 3)
+            __builtin_amdgcn_s_setprio(0);
+          else
+            __builtin_amdgcn_s_setprio(1);
+        }
         // s: this block's scores, s2: the next one's.  K of the next block at kat, V of this one at vat; K of the one after next goes to
         // kst, V of the next one to vst.
         if (SOFTCAP) {
@@ -918,11 +974,11 @@ __device__ __forceinline__ void kv4_tiled_impl(const Kv4AttnArgs& a) {
 
       // ---- out: lane (n, h) holds 4 consecutive d of row n in each group of four registers
       const bool whole = nj == nblk;
-      const int64_t slot = 2 * (int64_t)blockIdx.x + (first ? 0 : 1);
+      kv4_note_item(a, w, nblk, nj, slot);
       const float ls = pair_sum(l);
       if (valid) {
         const float inv = !whole ? 1.0f : ls != 0.0f ? 1.0f / ls : 0.0f;   // no visible key: 0
-        const int64_t pr = slot * a.tile_rows + (row - row0);
+        const int64_t pr = (int64_t)slot * a.tile_rows + (row - row0);
 #pragma unroll
         for (int j = 0; j < ND; j++)
 #pragma unroll
@@ -932,18 +988,18 @@ __device__ __forceinline__ void kv4_tiled_impl(const Kv4AttnArgs& a) {
             if (!whole)
               *reinterpret_cast<float4*>(a.part_o + pr * D + d) = x;
             else
-              kv4_store4(a, b, kvh, row, d, x);
+              kv4_store4(a, b, hd, qi, d, x);
           }
         if (!whole && h == 0) reinterpret_cast<float2*>(a.part_ml)[pr] = make_float2(mc, ls);
       }
     }
-    u0 += take;
-    if (u0 >= u1) return;
+    w.left -= take;
+    if (w.left <= 0) return;
     first = false;
-    in += take;
-    if (in == room * a.Hkv) {
-      in = 0;
-      gt++;
+    w.j0 = 0;
+    if (++w.kvh == a.Hkv) {
+      w.kvh = 0;
+      if (++w.gt == a.B * a.n_rt) return;
     }
   }
 }
@@ -960,56 +1016,81 @@ MXFA_KV4_TILED_ALL(128, 2)
 MXFA_KV4_TILED_ALL(256, 1)
 
 // The merge of the pieces of an item that several workgroups hold: O = sum O_p 2^(m_p - M) / sum l_p 2^(m_p -
-// M); 0 where nothing was visible.  A workgroup takes merge_rows rows of an item, D / 4 lanes of 4 d for each
-// of 256 / (D / 4) / merge_rows groups that take a row's pieces in turn: one row after the streaming form, whose
-// few rows may have a piece in every workgroup, as many as there are lanes for after the tiled one.
+// M); 0 where nothing was visible.  D / 4 lanes hold 4 d each of a row; merge_grp groups of them (a power of two) take
+// the row's pieces in turn, the workgroup's other lanes other rows: all lanes for one row after the streaming
+// form, where a row may have a piece in every workgroup, one group after the tiled one, whose rows are many
+// and have two or three.  blockIdx.y takes a part of the item's rows.  What bounds it is the latency of its loads, one after
+// the other: the arguments, the item's note, and the pieces (8 at a time, each group by its own maximum).
 extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_combine(Kv4AttnArgs a) {
   __shared__ __attribute__((aligned(16))) float so[256 * 4];
-  __shared__ float sl[16];
-  const int D = a.D, lanes = D / 4, tid = threadIdx.x, x = tid % lanes, ngrp = 256 / lanes / a.merge_rows;
-  const int grp = tid / lanes % ngrp, lane = tid & 63;
-  const int per = (min(a.tile_rows, a.rows) + a.merge_rows - 1) / a.merge_rows;
-  const int item = blockIdx.x / per, gt = item / a.Hkv, kvh = item % a.Hkv;
-  const int rr = blockIdx.x % per * a.merge_rows + tid / lanes / ngrp;   // row in the tile
+  __shared__ float2 sml[16];
+  const int2 item = reinterpret_cast<const int2*>(a.pieces)[blockIdx.x];
+  const int slot0 = item.x, np = item.y;
+  if (np == 1) return;                     // (written by its workgroup)
+  const int lanes = a.D / 4, tid = threadIdx.x, x = tid % lanes, ngrp = a.merge_grp, nrow = 256 / lanes / ngrp;
+  const int grp = tid / lanes % ngrp;
+  const int gt = blockIdx.x / a.Hkv, kvh = blockIdx.x % a.Hkv;
   int b, row0, i0, i1;
   kv4_tile(a, gt, b, row0, i0, i1);
-  const int share = kv4_share(a, kv4_line(a, lane, a.B * a.n_rt));
-  const int nblk = kv4_blocks(a, gt), start = kv4_line(a, lane, gt) + kvh * kv4_room(nblk);
-  const int w0 = start / share, np = (start + nblk - 1) / share - w0 + 1;
-  if (np == 1) return;                     // (written by its workgroup)
-  const int r = row0 + rr;
-  const bool have = rr < a.tile_rows && r < a.rows;
-  // piece p lies in slot 2 (w0 + p); the first one in 2 w0 + 1 where its workgroup's share begins before it
-  const int odd = start % share ? 1 : 0;
-  const float2* ml = reinterpret_cast<const float2*>(a.part_ml);
-  auto at = [&](int p) { return (int64_t)(2 * (w0 + p) + (p == 0 ? odd : 0)) * a.tile_rows + rr; };
-  float M = -INFINITY, L = 0.0f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (have) {
-#pragma unroll 4
-    for (int p = 0; p < np; p++) M = fmaxf(M, ml[at(p)].x);
-    const float m0 = M == -INFINITY ? 0.0f : M;
-#pragma unroll 4
-    for (int p = grp; p < np; p += ngrp) {
-      const float2 v = ml[at(p)];
-      const float4 o = *reinterpret_cast<const float4*>(a.part_o + at(p) * D + 4 * x);
-      const float w = __builtin_amdgcn_exp2f(v.x - m0);
-      L += v.y * w;
-      acc.x += o.x * w; acc.y += o.y * w; acc.z += o.z * w; acc.w += o.w * w;
+  const int rows = min(a.tile_rows, a.rows - row0);
+  const int slot1 = a.cut ? slot0 : slot0 & ~1, per = a.cut ? 1 : 2;
+  constexpr int CH = 8;
+  for (int r0 = blockIdx.y * nrow; r0 < rows; r0 += gridDim.y * nrow) {
+    const int rr = r0 + tid / lanes / ngrp;   // row in the tile
+    const bool have = rr < rows;
+    float M = -INFINITY, L = 0.0f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = grp; p0 < np; p0 += CH * ngrp) {
+      float2 v[CH];
+      float4 o[CH];
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        const int p = p0 + i * ngrp;
+        v[i] = make_float2(-INFINITY, 0.f);
+        o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < np) {
+          const int64_t at = (int64_t)(p ? slot1 + per * p : slot0) * a.tile_rows + (have ? rr : 0);
+          v[i] = reinterpret_cast<const float2*>(a.part_ml)[at];
+          o[i] = *reinterpret_cast<const float4*>(a.part_o + at * a.D + 4 * x);
+        }
+      }
+      float top = M;
+#pragma unroll
+      for (int i = 0; i < CH; i++) top = fmaxf(top, v[i].x);
+      const float m0 = top == -INFINITY ? 0.0f : top, old = __builtin_amdgcn_exp2f(M - m0);
+      M = top;
+      L *= old;
+      acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+#pragma unroll
+      for (int i = 0; i < CH; i++) {
+        const float w = __builtin_amdgcn_exp2f(v[i].x - m0);
+        L += v[i].y * w;
+        acc.x += o[i].x * w; acc.y += o[i].y * w; acc.z += o[i].z * w; acc.w += o[i].w * w;
+      }
     }
-  }
-  if (ngrp > 1) {
-    *reinterpret_cast<float4*>(&so[4 * tid]) = acc;
-    if (x == 0) sl[tid / lanes] = L;
-    __syncthreads();
-    if (grp) return;
-    for (int i = 1; i < ngrp; i++) {
-      const float4 o = *reinterpret_cast<const float4*>(&so[4 * (tid + i * lanes)]);
-      acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
-      L += sl[tid / lanes + i];
+    if (ngrp > 1) {
+      __syncthreads();                     // (the last row's sums have been read)
+      *reinterpret_cast<float4*>(&so[4 * tid]) = acc;
+      if (x == 0) sml[tid / lanes] = make_float2(M, L);
+      __syncthreads();
+      if (grp == 0) {
+        const int g0 = tid / lanes;
+        float top = M;
+        for (int i = 1; i < ngrp; i++) top = fmaxf(top, sml[g0 + i].x);
+        const float m0 = top == -INFINITY ? 0.0f : top;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        L = 0.0f;
+        for (int i = 0; i < ngrp; i++) {
+          const float4 o = *reinterpret_cast<const float4*>(&so[4 * (tid + i * lanes)]);
+          const float w = __builtin_amdgcn_exp2f(sml[g0 + i].x - m0);
+          L += sml[g0 + i].y * w;
+          acc.x += o.x * w; acc.y += o.y * w; acc.z += o.z * w; acc.w += o.w * w;
+        }
+      }
     }
+    if (grp || !have) continue;
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    const int r = row0 + rr, qi = r / a.group;
+    kv4_store4(a, b, kvh * a.group + r - qi * a.group, qi, 4 * x, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
   }
-  if (!have) return;
-  const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-  kv4_store4(a, b, kvh, r, 4 * x, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
 }

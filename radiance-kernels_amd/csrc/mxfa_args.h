@@ -80,8 +80,9 @@ struct Kv4AttnArgs {
   const uint8_t* vs;
   const int* kv_len;  // keys of each sequence [B], or NULL: Sk
   uint8_t* o;         // bf16 or fp32
-  float* part_o;      // [2 n_wg slots][tile_rows][D], unnormalized
-  float* part_ml;     // [2 n_wg slots][tile_rows][2]: the reference exponent (log2 units) and the row sum
+  float* part_o;      // [slots: n_wg if cut, else 2 n_wg][tile_rows][D], unnormalized
+  int* pieces;        // [items][2]: an item's first slot and the number of its pieces
+  float* part_ml;     // [slots][tile_rows][2]: the reference exponent (log2 units) and the row sum
   int64_t q_b, q_h, q_t, o_b, o_h, o_t;   // element strides
   int B, Hq, Hkv, Sq, Sk, L;
   int group, rows;    // Hq / Hkv; rows of a KV head: group * Sq, row r = query r / group of head r % group
@@ -89,7 +90,10 @@ struct Kv4AttnArgs {
   int D, n_rt, tile_rows;   // row tiles of a KV head and their rows
   int n_wg;           // workgroups that share the blocks of all items; 0: one workgroup per item
   int min_share;      // blocks of a workgroup's share at least
-  int merge_rows;     // rows of a workgroup of the merge
+  int cut;            // each item cut into pieces, a workgroup each (else shares of the line of all items)
+  int wg_log2;        // log2 n_wg
+  int group_inv;      // ceil(2^16 / group): r * it >> 16 is r / group for r < 32
+  int merge_grp;      // groups of a workgroup of the merge that share a row's pieces
   float c_log2, sc_u, cap_log2;
 };
 

@@ -1030,7 +1030,8 @@ mxfa_status check_kv4_attn(const mxfa_kv4_attn_params* p) {
 // workgroup per item or equal shares of the line of all items' blocks (kv4_my_share in k_kv4.hip).
 struct Kv4Plan {
   bool tiled;
-  int n_rt, tile_rows, n_wg, min_share;
+  int n_rt, tile_rows, n_wg, min_share, slots;
+  bool cut;
   int64_t items;           // (sequence, row tile, KV head)
   size_t ws;
 };
@@ -1052,7 +1053,9 @@ mxfa_status kv4_plan(const mxfa_kv4_attn_params* p, Kv4Plan* out) {
   const int slots = p->head_dim == 256 && rows > 16 ? 256 : 512;
   const bool per_item = blocks <= 2 * out->min_share || out->items >= 8 * slots;
   out->n_wg = per_item ? 0 : slots;
-  out->ws = per_item ? 0 : (size_t)2 * out->n_wg * out->tile_rows * (p->head_dim + 2) * sizeof(float);
+  out->cut = 2 * out->items <= out->n_wg;
+  out->slots = out->cut ? out->n_wg : 2 * out->n_wg;
+  out->ws = out->n_wg ? (size_t)out->slots * out->tile_rows * (p->head_dim + 2) * sizeof(float) + (size_t)out->items * 8 : 0;
   return MXFA_OK;
 }
 
@@ -1107,26 +1110,33 @@ mxfa_status mxfa_kv4_attention(const mxfa_kv4_attn_params* p, const void* q, con
   a.kv_len = kv_len; a.o = static_cast<uint8_t*>(o);
   a.B = p->batch; a.Hq = p->num_q_heads; a.Hkv = p->num_kv_heads; a.Sq = p->seq_q; a.Sk = p->seq_k; a.L = p->max_len;
   a.group = p->num_q_heads / p->num_kv_heads;
+  a.group_inv = (65535 + a.group) / a.group;
   a.rows = a.group * p->seq_q;
   a.q_pos0 = p->q_pos0;
   a.window = p->window < (1 << 30) ? p->window : 0;              // (positions stay below 2^30: no key is that far behind)
   a.causal = p->causal != 0;
   a.o_bf16 = bf16;
-  a.D = p->head_dim; a.n_rt = plan.n_rt; a.tile_rows = plan.tile_rows; a.n_wg = plan.n_wg; a.min_share = plan.min_share;
-  a.merge_rows = plan.tiled ? 1024 / p->head_dim : 1;
+  a.D = p->head_dim; a.n_rt = plan.n_rt; a.tile_rows = plan.tile_rows; a.n_wg = plan.n_wg; a.min_share = plan.min_share; a.cut = plan.cut;
+  while (plan.n_wg >> (a.wg_log2 + 1)) a.wg_log2++;
   const float log2e = 1.4426950408889634f;
   a.c_log2 = p->softmax_scale * log2e;
   if (p->softcap > 0.0f) {
     a.sc_u = p->softmax_scale / p->softcap;
     a.cap_log2 = p->softcap * log2e;
   }
+  // the merge: as many groups to a row as it has pieces on average, up to a workgroup's 1024 / D, and about 1,024
+  // workgroups (20 rows of 128 items, us: 18.0 in 256 workgroups of one row at a time, 6.2 so)
+  a.merge_grp = 1;
+  while (!plan.tiled && a.merge_grp < 1024 / p->head_dim && (int64_t)a.merge_grp * plan.items < plan.n_wg + plan.items) a.merge_grp *= 2;
+  const int64_t merge_rows = 1024 / p->head_dim / a.merge_grp, tile = std::min(plan.tile_rows, a.rows);
+  const int64_t merge_y = std::max<int64_t>(1, std::min<int64_t>((tile + merge_rows - 1) / merge_rows, (plan.tiled ? 4096 : 1024) / plan.items));
   if (plan.n_wg) {
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + (size_t)2 * plan.n_wg * plan.tile_rows * p->head_dim;
+    a.part_ml = a.part_o + (size_t)plan.slots * plan.tile_rows * p->head_dim;
+    a.pieces = reinterpret_cast<int*>(a.part_ml + (size_t)plan.slots * plan.tile_rows * 2);
   }
-  const int64_t grid = plan.n_wg ? plan.n_wg : plan.items, merge = plan.n_wg ? plan.items * ((std::min(plan.tile_rows, a.rows) + a.merge_rows - 1) / a.merge_rows) : 0;
-  if (mxfa_status st = check_grid(grid, 256)) return st;
-  if (mxfa_status st = check_grid(merge, 256)) return st;
+  const int64_t grid = plan.n_wg ? plan.n_wg : plan.items;
+  if (mxfa_status st = check_grid(std::max(grid, plan.items), 256)) return st;
   DeviceModule* dm;
   if (mxfa_status st = module_for_current(&dm)) return st;
   char name[48];
@@ -1135,7 +1145,7 @@ mxfa_status mxfa_kv4_attention(const mxfa_kv4_attn_params* p, const void* q, con
   void* args[] = {&a};
   if (mxfa_status st = launch(dm, name, dim3((unsigned)grid), dim3(256), args, stream)) return st;
   if (!plan.n_wg) return MXFA_OK;
-  return launch(dm, "mxfa_kv4_combine", dim3((unsigned)merge), dim3(256), args, stream);
+  return launch(dm, "mxfa_kv4_combine", dim3((unsigned)plan.items, (unsigned)merge_y), dim3(256), args, stream);
 }
 
 mxfa_status mxfa_rmsnorm_quantize(const mxfa_norm_params* p, const void* x, const void* residual, const void* weight, void* h,
