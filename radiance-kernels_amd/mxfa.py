@@ -465,8 +465,20 @@ class KvCache:
 
 # ---- 4-bit KV cache (mxfa_kv4_*) and the norm in front of a projection -------------------------
 
+class _Torch:
+    """torch, imported at its first use; the name then holds the module itself (an import statement in each of a
+    call's checks cost a microsecond per call)."""
+
+    def __getattr__(self, name):
+        global torch
+        import torch
+        return getattr(torch, name)
+
+
+torch = _Torch()
+
+
 def _x_fmt(t, name):
-    import torch
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise MxfaError(1, f"{name} must be a CUDA tensor")
     if t.dtype is torch.bfloat16:
@@ -479,8 +491,7 @@ def _x_fmt(t, name):
 def _rows(t, dtype, shape, device, name, written=False):
     """mxfa_strides of a [B, H, n, D] tensor whose rows of D are contiguous (None: dense), after a check of its
     device, dtype and shape.  written: rows must not share memory."""
-    import torch
-    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.device == device):
+    if not (isinstance(t, torch.Tensor) and t.get_device() == device.index):
         raise MxfaError(1, f"{name} must be a tensor on {device}")
     if t.dtype is not dtype:
         raise MxfaError(1, f"{name} must be {dtype}, got {t.dtype}")
@@ -502,18 +513,16 @@ def _rows(t, dtype, shape, device, name, written=False):
 
 def _index(t, n, device, name):
     """Pointer of an int32 [n] tensor on `device`, or None."""
-    import torch
     if t is None:
         return None
-    if not (isinstance(t, torch.Tensor) and t.device == device and t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()):
+    if not (isinstance(t, torch.Tensor) and t.get_device() == device.index and t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()):
         raise MxfaError(1, f"{name} must be a contiguous int32 tensor of shape ({n},) on {device}")
     return t.data_ptr()
 
 
 def _on(device):
     """The library launches on the current device: a call whose tensors lie elsewhere is refused."""
-    import torch
-    if device.index != torch.cuda.current_device():
+    if device.index != torch._C._cuda_getDevice():
         raise MxfaError(1, f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
@@ -567,7 +576,6 @@ class Kv4Cache:
     def read(self, n, pos=0, dtype=None, out=None, stream=None):
         """(K, V) [B, Hkv, n, D], bfloat16 (default) or float32: the values of n tokens from `pos` (an int, or an
         int32 CUDA tensor [B]) on.  out: a pair of tensors to write, rows contiguous, the other strides free."""
-        import torch
         c, dev = self.shape, self.k.device
         shape = (c.batch, c.num_kv_heads, n, c.head_dim)
         if out is None:
@@ -601,7 +609,6 @@ def kv4_attention(p, q, cache, kv_len=None, out=None, workspace=None, stream=Non
     """O of new queries over a Kv4Cache (mxfa_kv4_attention): q bfloat16 [B, Hq, Sq, D] and out [B, Hq, Sq, D] of
     p.o_fmt, rows contiguous, the other strides free; kv_len: int32 CUDA tensor [B], each sequence's keys
     (None: p.seq_k, queries from p.q_pos0 on).  workspace: a uint8 tensor of kv4_attention_plan's bytes."""
-    import torch
     c, dev = cache.shape, cache.k.device
     if (p.batch, p.num_kv_heads, p.head_dim, p.max_len) != (c.batch, c.num_kv_heads, c.head_dim, c.max_len):
         raise MxfaError(1, "the parameters' batch, num_kv_heads, head_dim and max_len are not the cache's")
@@ -624,8 +631,7 @@ def rmsnorm_quantize(x, weight, eps=1e-6, residual=None, weight_offset=0.0, gemm
     """(codes, scales, h) of mxfa_rmsnorm_quantize: x [..., cols] float32 or bfloat16, contiguous; residual like x or
     None (h is then x itself); h: where x + residual goes (residual or x for in place; None allocates).
     gemm_scales: scales [cols/32, rows], gemm's A scales, else [..., cols/32]."""
-    import torch
-    fmt = _x_fmt(x, "x")
+    fmt, dev = _x_fmt(x, "x"), x.device
     cols = x.shape[-1] if x.dim() else 0
     if cols < 32 or cols % 32:
         raise MxfaError(1, "cols must be a positive multiple of 32")
@@ -641,11 +647,11 @@ def rmsnorm_quantize(x, weight, eps=1e-6, residual=None, weight_offset=0.0, gemm
             h = torch.empty_like(x)
         _need(h, x.dtype, x.shape, "h")
     for t, name in ((weight, "weight"), (residual, "residual"), (h, "h")):
-        if t is not None and t.device != x.device:
-            raise MxfaError(1, f"{name} must be on {x.device}")
-    _on(x.device)
-    codes = torch.empty(x.shape, dtype=torch.uint8, device=x.device)
-    scales = torch.empty((cols // 32, rows) if gemm_scales else (*x.shape[:-1], cols // 32), dtype=torch.uint8, device=x.device)
+        if t is not None and t.get_device() != dev.index:
+            raise MxfaError(1, f"{name} must be on {dev}")
+    _on(dev)
+    codes = torch.empty_like(x, dtype=torch.uint8)
+    scales = torch.empty((cols // 32, rows) if gemm_scales else (*x.shape[:-1], cols // 32), dtype=torch.uint8, device=dev)
     p = NormParams(rows, cols, fmt, float(eps), float(weight_offset), rows if gemm_scales else 0)
     _check(lib().mxfa_rmsnorm_quantize(p, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(h),
                                        codes.data_ptr(), scales.data_ptr(), _stream(stream)))
