@@ -201,18 +201,9 @@ __device__ __forceinline__ float col_max(float x) {
 struct Kv4Seq {
   int len, pos0;
 };
-// UNIFORM: b is the same in all lanes (the length then lives in scalar registers, also where stores lie between).
-template <bool UNIFORM>
-__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int b) {
-  Kv4Seq s;
-  s.len = a.Sk;
-  if (a.kv_len) {
-    const int len = a.kv_len[b];
-    s.len = min(max(UNIFORM ? __builtin_amdgcn_readfirstlane(len) : len, 0), a.Sk);
-  }
-  s.pos0 = a.kv_len ? s.len - a.Sq : a.q_pos0;
-  return s;
-}
+// Keys of sequence b.
+__device__ __forceinline__ int kv4_len(const Kv4AttnArgs& a, int b) { return a.kv_len ? min(max(a.kv_len[b], 0), a.Sk) : a.Sk; }
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttnArgs& a, int len) { return {len, a.kv_len ? len - a.Sq : a.q_pos0}; }
 __device__ __forceinline__ void kv4_limits(const Kv4AttnArgs& a, Kv4Seq s, int i, int& lo, int& hi) {
   hi = a.causal ? min(s.len - 1, s.pos0 + i) : s.len - 1;
   lo = a.window > 0 ? max(0, s.pos0 + i - a.window + 1) : 0;
@@ -227,15 +218,15 @@ __device__ __forceinline__ void kv4_tile(const Kv4AttnArgs& a, int gt, int& b, i
   i0 = a.n_rt == 1 ? 0 : row0 / a.group;
   i1 = a.n_rt == 1 ? a.Sq - 1 : (min(row0 + a.tile_rows, a.rows) - 1) / a.group;
 }
-template <bool UNIFORM>
-__device__ __forceinline__ int kv4_blocks(const Kv4AttnArgs& a, int gt) {
+__device__ __forceinline__ int kv4_blocks(const Kv4AttnArgs& a, int gt, int len) {
   int b, row0, i0, i1, lo, hi, t;
   kv4_tile(a, gt, b, row0, i0, i1);
-  const Kv4Seq s = kv4_seq<UNIFORM>(a, b);
+  const Kv4Seq s = kv4_seq(a, len);
   kv4_limits(a, s, i0, lo, t);
   kv4_limits(a, s, i1, t, hi);
   return hi >= lo ? hi / KV4_BK - lo / KV4_BK + 1 : 1;
 }
+__device__ __forceinline__ int kv4_tile_len(const Kv4AttnArgs& a, int gt) { return kv4_len(a, a.n_rt == 1 ? gt : gt / a.n_rt); }
 // What an item takes up in the line: its blocks and, short ones, room for the time that a piece costs by itself
 // (Q, the first loads, the merge: some 8 blocks' worth), so that a share does not hold many of them.
 __device__ __forceinline__ int kv4_room(int nblk) { return nblk < 32 ? nblk + 8 : nblk; }
@@ -263,7 +254,7 @@ __device__ __forceinline__ uint32_t kv4_share(const Kv4AttnArgs& a, int lane, ui
   const int groups = a.B * a.n_rt;
   auto sum = [&](auto f) {
     uint32_t n = nblk0 ? f(nblk0) : 0;
-    for (int gt = 64 + lane; gt < groups; gt += 64) n += f(kv4_blocks<false>(a, gt));
+    for (int gt = 64 + lane; gt < groups; gt += 64) n += f(kv4_blocks(a, gt, kv4_tile_len(a, gt)));
     return __builtin_amdgcn_readlane(wave_prefix(n), 63) * (uint32_t)a.Hkv;
   };
   const uint32_t total = sum([&](uint32_t n) { return a.cut ? n : kv4_room(n); });
@@ -276,24 +267,29 @@ __device__ __forceinline__ uint32_t kv4_share(const Kv4AttnArgs& a, int lane, ui
 }
 
 // This workgroup's part of the line: `left` places from j0 of item (row tile gt, KV head kvh) on; an item's later pieces
-// hold `share`.  False: none.
+// hold `share`; len: its keys.  False: none.
 struct Kv4Part {
-  int gt, kvh, j0, left, share;
+  int gt, kvh, j0, left, share, len;
 };
 __device__ __forceinline__ bool kv4_my_part(const Kv4AttnArgs& a, int lane, Kv4Part& w) {
   if (!a.n_wg) {                           // one workgroup per item, the tiles that see most keys first
     w.gt = a.B * a.n_rt - 1 - blockIdx.x / a.Hkv;
     w.kvh = blockIdx.x % a.Hkv;
     w.j0 = 0;
-    w.left = w.share = kv4_room(kv4_blocks<true>(a, w.gt));
+    w.len = __builtin_amdgcn_readfirstlane(kv4_tile_len(a, w.gt));
+    w.left = w.share = kv4_room(kv4_blocks(a, w.gt, w.len));
     return true;
   }
   const int groups = a.B * a.n_rt;
-  uint32_t nblk = lane < groups ? kv4_blocks<false>(a, lane) : 0;
+  int len = kv4_tile_len(a, min(lane, groups - 1));
+  uint32_t nblk = lane < groups ? kv4_blocks(a, lane, len) : 0;
   const uint32_t share = kv4_share(a, lane, nblk), u0 = a.cut ? blockIdx.x : blockIdx.x * share;
   uint32_t at = 0;                         // places (cut: pieces) before tile g0
   for (int g0 = 0; g0 < groups; g0 += 64) {
-    if (g0) nblk = g0 + lane < groups ? kv4_blocks<false>(a, g0 + lane) : 0;
+    if (g0) {
+      len = kv4_tile_len(a, min(g0 + lane, groups - 1));
+      nblk = g0 + lane < groups ? kv4_blocks(a, g0 + lane, len) : 0;
+    }
     const uint32_t each = !nblk ? 0 : a.cut ? kv4_pieces(nblk, share) : kv4_room(nblk), mine = each * a.Hkv;
     const uint32_t sum = wave_prefix(mine);
     const uint64_t past = __ballot(at + sum > u0);
@@ -302,6 +298,7 @@ __device__ __forceinline__ bool kv4_my_part(const Kv4AttnArgs& a, int lane, Kv4P
       const uint32_t n = __builtin_amdgcn_readlane(nblk, l), per = __builtin_amdgcn_readlane(each, l);
       const uint32_t in = u0 - (at + __builtin_amdgcn_readlane(sum, l) - per * a.Hkv);
       w.gt = g0 + l;
+      w.len = __builtin_amdgcn_readlane(len, l);
       w.kvh = in / per;
       w.j0 = in - w.kvh * per;
       w.left = w.share = share;            // (the walk ends at the last tile)
@@ -354,12 +351,12 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
   bool first = true;
 
   while (true) {
-    const int nblk = kv4_blocks<true>(a, w.gt), b = w.gt, kvh = w.kvh, j0 = w.j0;       // (one row tile)
+    const int nblk = kv4_blocks(a, w.gt, w.len), b = w.gt, kvh = w.kvh, j0 = w.j0;       // (one row tile)
     const int take = min(kv4_room(nblk) - j0, w.left), nj = min(nblk - j0, take);
     if (nj > 0) {
     const int slot = a.cut ? blockIdx.x : 2 * blockIdx.x + (first ? 0 : 1);
     const int bk = b * a.Hkv + kvh;
-    const Kv4Seq seq = kv4_seq<true>(a, b);
+    const Kv4Seq seq = kv4_seq(a, w.len);
     // each column's keys, and those that every column sees or any does
     int klo[NT], khi[NT], klo_all, khi_all, klo_any, khi_any;
     kv4_limits(a, seq, 0, klo_any, khi_all);
@@ -648,6 +645,7 @@ __device__ __forceinline__ void kv4_attn_impl(const Kv4AttnArgs& a) {
     if (++w.kvh == a.Hkv) {
       w.kvh = 0;
       if (++w.gt == a.B * a.n_rt) return;
+      w.len = __builtin_amdgcn_readfirstlane(kv4_tile_len(a, w.gt));
     }
   }
 }
@@ -700,14 +698,14 @@ __device__ __forceinline__ void kv4_tiled_impl(const Kv4AttnArgs& a) {
   bool first = true;
 
   while (true) {
-    const int nblk = kv4_blocks<true>(a, w.gt), kvh = w.kvh, j0 = w.j0;
+    const int nblk = kv4_blocks(a, w.gt, w.len), kvh = w.kvh, j0 = w.j0;
     const int take = min(kv4_room(nblk) - j0, w.left), nj = min(nblk - j0, take);
     if (nj > 0) {
       const int slot = a.cut ? blockIdx.x : 2 * blockIdx.x + (first ? 0 : 1);
       int b, row0, i0, i1;
       kv4_tile(a, w.gt, b, row0, i0, i1);
       const int bk = b * a.Hkv + kvh;
-      const Kv4Seq seq = kv4_seq<true>(a, b);
+      const Kv4Seq seq = kv4_seq(a, w.len);
       int klo_any, khi_any, t0, t1;
       kv4_limits(a, seq, i0, klo_any, t0);
       kv4_limits(a, seq, i1, t1, khi_any);
@@ -1000,6 +998,7 @@ __device__ __forceinline__ void kv4_tiled_impl(const Kv4AttnArgs& a) {
     if (++w.kvh == a.Hkv) {
       w.kvh = 0;
       if (++w.gt == a.B * a.n_rt) return;
+      w.len = __builtin_amdgcn_readfirstlane(kv4_tile_len(a, w.gt));
     }
   }
 }
