@@ -1039,6 +1039,8 @@ struct Kv4Plan {
 mxfa_status kv4_plan(const mxfa_kv4_attn_params* p, Kv4Plan* out) {
   const int64_t rows = (int64_t)(p->num_q_heads / p->num_kv_heads) * p->seq_q;
   const int64_t bk = (int64_t)p->batch * p->num_kv_heads, blocks = (p->seq_k + 63) / 64;
+  // (16 sequences of 8,192 tokens, 8 KV heads of D = 128, 32 rows: streaming 48 us, tiled 81; D = 256, 20 rows, 4 KV
+  // heads: 50 and 105.  Above 32 rows the streaming form has no registers left.)
   out->tiled = rows > 32;
   out->tile_rows = out->tiled ? 128 : rows <= 16 ? 16 : 32;
   out->n_rt = (int)((rows + out->tile_rows - 1) / out->tile_rows);
@@ -1046,13 +1048,22 @@ mxfa_status kv4_plan(const mxfa_kv4_attn_params* p, Kv4Plan* out) {
   if (bk > (int64_t)INT32_MAX / 256 / out->n_rt || bk * out->n_rt > (int64_t)INT32_MAX / (blocks + 8))
     return fail(MXFA_ERR_UNSUPPORTED, "the call walks more than 2^31 blocks of keys: split it");
   out->items = bk * out->n_rt;
-  // One workgroup per item for short caches, where a share would be a piece too small to pay for its merge, and for so
-  // many items that their different lengths even out; else as many shares as workgroups fit the chip at once: two
-  // per CU, at D = 256 with more than 16 rows one.
+  // As many shares as workgroups fit the chip at once: two per CU, at D = 256 with more than 16 rows one.
+  // (min_share, streaming, 8 KV heads: 4,096 tokens 10.1, 11.0, 13.0 us with 4, 8, 16; 16,384 tokens 12.8, 12.2, 14.2)
+  const int64_t slots = p->head_dim == 256 && rows > 16 ? 256 : 512;
   out->min_share = 8;
-  const int slots = p->head_dim == 256 && rows > 16 ? 256 : 512;
-  const bool per_item = blocks <= 2 * out->min_share || out->items >= 8 * slots;
-  out->n_wg = per_item ? 0 : slots;
+  // Or one workgroup per item: for short caches, where a share would be a piece too small to pay for its merge (2 x
+  // 8 items of 16 blocks 9.0 us against 11.1; of 32 blocks 14.8 against 11.5), and where what idles at the end, about
+  // half an item's time (lengths may differ) or what the last round leaves empty, costs less than the merge and the
+  // second pieces.  Those cost 8 + 8 per round in a streamed block's time, 16 + 16 in a tiled one's.  Us, items
+  // against shares (r: ragged):
+  //   streaming: 512 items of 32 blocks r 21.4, 25.5; 2,048 of 32 r 63, 73; of 128 r 197, 188; 4,096 of 128 r 368, 373
+  //   tiled: 512 items of 64 blocks 144, 171; 2,048 of 64 295, 353; 640 of 64 228, 213; 512 of 256 r 406, 330
+  const int64_t seen = p->window > 0 ? std::min(blocks, ((int64_t)p->window + std::min<int64_t>(p->seq_q, out->tile_rows)) / 64 + 2) : blocks;
+  const int64_t left = (slots - out->items % slots) % slots;
+  const bool per_item = seen <= 2 * out->min_share ||
+                        std::max(2 * left, slots) * seen <= (out->tiled ? 32 : 16) * (slots + out->items);
+  out->n_wg = per_item ? 0 : (int)slots;
   out->cut = 2 * out->items <= out->n_wg;
   out->slots = out->cut ? out->n_wg : 2 * out->n_wg;
   out->ws = out->n_wg ? (size_t)out->slots * out->tile_rows * (p->head_dim + 2) * sizeof(float) + (size_t)out->items * 8 : 0;
