@@ -290,6 +290,40 @@ def test_attention_split_over_a_long_cache(B, Hq, Hkv, Sq, D, n, kw, f32):
     _check(got, _want(q, cache, lens, p, False), p, n, f"{shares} shares")
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,D,n,kw,line", [
+    (100, 2, 1, 1, 64, 1200, {}, False),                         # pieces of items, more tiles than a wave has lanes
+    (80, 8, 4, 1, 64, 1900, {}, True),                           # a line of items cut into shares
+    (40, 16, 8, 1, 128, 1900, dict(window=1700), True),
+    (68, 8, 4, 9, 64, 1900, {}, True),                           # (two tiles of rows)
+    (24, 16, 4, 66, 64, 3300, {}, True),                         # (tiled, three row tiles to a KV head)
+    (34, 4, 2, 80, 256, 3300, dict(softcap=30.0), True),
+])
+def test_attention_of_many_items(B, Hq, Hkv, Sq, D, n, kw, line):
+    """Ragged batches whose items are shared out over workgroups: lengths of 0, 1 and around a block's end, and one
+    in four long, so that a share ends inside an item, holds many, or none."""
+    print(f"many B{B} Hq{Hq} Hkv{Hkv} Sq{Sq} D{D} n{n} {kw}", flush=True)
+    L = (n + 31) // 32 * 32
+    rng = np.random.default_rng(B + Sq)
+    lens = [int(x) for x in np.where(np.arange(B) % 4 == 1, rng.integers(n // 2, n + 1, B), rng.integers(0, 200, B))]
+    lens[0], lens[2], lens[3], lens[4], lens[6], lens[-1] = 0, 1, 63, 64, 65, n
+    q, cache, lt = _problem(B, Hq, Hkv, Sq, D, L, lens, seed=n + Sq, amp=1.5)
+    p = mxfa.make_kv4_params(B, Hq, Hkv, Sq, n, D, L, **kw)
+    shares, ws = mxfa.kv4_attention_plan(p)
+    rows = Hq // Hkv * Sq
+    slots = ws // (4 * (D + 2) * (16 if rows <= 16 else 32 if rows <= 32 else 128))
+    assert shares > 1 and slots == (2 * shares if line else shares)
+    full = torch.full((ws,), 255, dtype=torch.uint8, device=DEV)
+    got = mxfa.kv4_attention(p, q, cache, kv_len=lt, workspace=full)
+    _check(got, _want(q, cache, lens, p, False), p, n, f"{shares} shares")
+    assert torch.equal(got, mxfa.kv4_attention(p, q, cache, kv_len=lt, workspace=full))
+    # an empty batch but for its last sequence
+    lens0 = [0] * (B - 1) + [n]
+    lt0 = torch.tensor(lens0, dtype=torch.int32, device=DEV)
+    last = mxfa.kv4_attention(p, q, cache, kv_len=lt0, workspace=full)
+    assert not bool(last[:-1].any())
+    _check(last, _want(q, cache, lens0, p, False), p, n, "the last alone")
+
+
 def test_attention_lengths_are_clamped():
     q, cache, _ = _problem(3, 4, 2, 1, 128, 96, [96, 96, 96], seed=4)
     p = mxfa.make_kv4_params(3, 4, 2, 1, 90, 128, 96)
