@@ -351,15 +351,16 @@ typedef struct {
   int32_t o_fmt;                            /* mxfa_c_fmt of O                                            */
 } mxfa_kv4_attn_params;
 
-/* n_shares: the equal shares into which the key blocks of all sequences and heads are cut, whatever their
- * lengths; what lies on both sides of a cut is merged through the workspace (0: no cuts, and
- * workspace_bytes is 0). */
+/* n_shares: the workgroups among which the key blocks of all sequences and heads are dealt, whatever their
+ * lengths; what several of them hold of a row is merged through the workspace (0: a workgroup walks all
+ * keys of its rows, and workspace_bytes is 0).  The plan depends on the parameters alone. */
 mxfa_status mxfa_kv4_attention_plan(const mxfa_kv4_attn_params *p, int32_t *n_shares, size_t *workspace_bytes);
 
 /* q: bf16 rows [B][Hq][seq_q][D] as q_strides say; o: bf16 or fp32 rows as o_strides say.  Scores and sums
  * are fp32, of the exact cache values; P enters the PV product as three bf16 terms for fp32 O (2^-24 of
  * P), for bf16 O as two up to 32 query rows of a KV head (2^-16) and one beyond (2^-8, as O itself is
- * rounded).  Calls that overlap need a workspace each. */
+ * rounded).  The sums are fp32: where |V| passes 2^123 / seq_k they may end in infinity.  Calls that
+ * overlap need a workspace each. */
 mxfa_status mxfa_kv4_attention(const mxfa_kv4_attn_params *p, const void *q, const mxfa_strides *q_strides,
                                const uint8_t *k_cache, const uint8_t *k_sc, const uint8_t *v_cache,
                                const uint8_t *v_sc, const int32_t *kv_len, void *o, const mxfa_strides *o_strides,

@@ -1016,6 +1016,10 @@ mxfa_status check_kv4_attn(const mxfa_kv4_attn_params* p) {
   if (!(p->softmax_scale > 0.0f) || !std::isfinite(p->softmax_scale))
     return fail(MXFA_ERR_INVALID_ARG, "softmax_scale must be finite and > 0");
   if (!(p->softcap >= 0.0f) || !std::isfinite(p->softcap)) return fail(MXFA_ERR_INVALID_ARG, "softcap must be finite and >= 0");
+  // (in log2 units, and the scale over the cap, which the kernels multiply by)
+  if (!std::isfinite(p->softmax_scale * 1.5f) || !std::isfinite(p->softcap * 1.5f) ||
+      (p->softcap > 0.0f && !std::isfinite(3.0f * (p->softmax_scale / p->softcap))))
+    return fail(MXFA_ERR_INVALID_ARG, "softmax_scale, softcap and their quotient must be finite in log2 units");
   if (p->o_fmt != MXFA_C_F32 && p->o_fmt != MXFA_C_BF16) return fail(MXFA_ERR_INVALID_ARG, "o_fmt must be MXFA_C_F32 or MXFA_C_BF16");
   // a (batch, KV head)'s codes are addressed with 32-bit byte offsets, positions with 32-bit sums
   if ((int64_t)p->max_len * (p->head_dim / 2) > (int64_t)INT32_MAX)

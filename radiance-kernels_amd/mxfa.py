@@ -526,14 +526,34 @@ def _on(device):
         raise MxfaError(1, f"the tensors are on {device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
+def _empty(shape, dtype, device, stream):
+    """A tensor for a call on `stream`, allocated there: memory of the current stream could still be in use there, or
+    be handed out again while the call runs."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def _int32(**values):
+    """The values as ints, refused where a 32-bit field would cut them."""
+    for name, v in values.items():
+        if not -2 ** 31 <= v < 2 ** 31:
+            raise MxfaError(1, f"{name} = {v} does not fit 32 bits")
+    return [int(v) for v in values.values()]
+
+
 class Kv4Cache:
     """A 4-bit KV cache on the device (layouts in mxfa.h).  Sequences may have lengths of their own: `pos` of
     append and read and kv_len of kv4_attention are then int32 CUDA tensors [batch], which the caller
     advances; without them append writes at `length`, the same for every sequence, and advances it."""
 
     def __init__(self, batch, num_kv_heads, head_dim, max_len, device="cuda:0"):
-        import torch
-        B, H, D, L = batch, num_kv_heads, head_dim, max_len
+        B, H, D, L = _int32(batch=batch, num_kv_heads=num_kv_heads, head_dim=head_dim, max_len=max_len)
+        if min(B, H) < 1 or D < 32 or D % 32 or L < 32 or L % 32:
+            raise MxfaError(1, "batch and num_kv_heads must be >= 1, head_dim and max_len positive multiples of 32")
         self.shape = Kv4Shape(B, H, D, L)
         self.k = torch.zeros((B, H, L, D // 2), dtype=torch.uint8, device=device)
         self.ks = torch.zeros((B, H, L // 32, 4, D // 32, 8), dtype=torch.uint8, device=device)
@@ -544,9 +564,10 @@ class Kv4Cache:
     @classmethod
     def of(cls, k, ks, v, vs, length=0):
         """A cache in tensors that exist: k, v [B, H, L, D/2] and ks, vs [B, H, L/32, 4, D/32, 8], uint8."""
-        import torch
         self = cls.__new__(cls)
-        B, H, L, half = k.shape
+        if not (isinstance(k, torch.Tensor) and k.dim() == 4):
+            raise MxfaError(1, "k must be a tensor [B, H, L, D/2]")
+        B, H, L, half = _int32(**dict(zip(("batch", "num_kv_heads", "max_len", "half"), k.shape)))
         for t, shape, name in ((k, (B, H, L, half), "k"), (ks, (B, H, L // 32, 4, half // 16, 8), "k_sc"),
                                (v, (B, H, L, half), "v"), (vs, (B, H, L // 32, 4, half // 16, 8), "v_sc")):
             _need(t, torch.uint8, shape, name)
@@ -557,8 +578,10 @@ class Kv4Cache:
         return self
 
     def append(self, k_new, v_new, pos=None, counts=None, stream=None):
-        """k_new, v_new: float32 or bfloat16 [B, Hkv, n, D], rows contiguous, the other strides free.  counts:
-        int32 CUDA tensor [B], of each sequence only the first counts[b] tokens are written."""
+        """k_new, v_new: float32 or bfloat16 [B, Hkv, n, D], rows contiguous, the other strides free.  counts (with
+        pos): int32 CUDA tensor [B], of each sequence only the first counts[b] tokens are written."""
+        if counts is not None and pos is None:
+            raise MxfaError(1, "counts needs pos: sequences of their own lengths have no common `length`")
         c, dev = self.shape, self.k.device
         fmt = _x_fmt(k_new, "k_new")
         shape = (c.batch, c.num_kv_heads, k_new.shape[2] if k_new.dim() == 4 else -1, c.head_dim)
@@ -577,16 +600,18 @@ class Kv4Cache:
         """(K, V) [B, Hkv, n, D], bfloat16 (default) or float32: the values of n tokens from `pos` (an int, or an
         int32 CUDA tensor [B]) on.  out: a pair of tensors to write, rows contiguous, the other strides free."""
         c, dev = self.shape, self.k.device
+        ragged = isinstance(pos, torch.Tensor)
+        if n < 0 or (not ragged and not 0 <= pos <= c.max_len - n):
+            raise MxfaError(1, f"read of {n} tokens at {pos}: the cache has {c.max_len}")
         shape = (c.batch, c.num_kv_heads, n, c.head_dim)
         if out is None:
-            out = tuple(torch.empty(shape, dtype=dtype or torch.bfloat16, device=dev) for _ in range(2))
+            out = tuple(_empty(shape, dtype or torch.bfloat16, dev, stream) for _ in range(2))
         K, V = out
         fmt = _x_fmt(K, "out[0]")
         if dtype is not None and K.dtype is not dtype:
             raise MxfaError(1, f"out[0] must be {dtype}, got {K.dtype}")
         ks, vs = _rows(K, K.dtype, shape, dev, "out[0]", True), _rows(V, K.dtype, shape, dev, "out[1]", True)
         _on(dev)
-        ragged = isinstance(pos, torch.Tensor)
         _check(lib().mxfa_kv4_read(c, fmt, self.k.data_ptr(), self.ks.data_ptr(), self.v.data_ptr(), self.vs.data_ptr(),
                                    _index(pos, c.batch, dev, "pos") if ragged else None, 0 if ragged else pos, n,
                                    K.data_ptr(), ks, V.data_ptr(), vs, _stream(stream)))
@@ -594,8 +619,8 @@ class Kv4Cache:
 
 
 def make_kv4_params(B, Hq, Hkv, Sq, Sk, D, max_len, causal=True, q_pos0=0, window=0, scale=None, softcap=0.0, o_fmt=C_BF16):
-    return Kv4AttnParams(B, Hq, Hkv, Sq, Sk, D, int(max_len), int(bool(causal)), int(q_pos0), int(window),
-                         float(scale if scale is not None else 1.0 / math.sqrt(D)), float(softcap), int(o_fmt))
+    ints = _int32(B=B, Hq=Hq, Hkv=Hkv, Sq=Sq, Sk=Sk, D=D, max_len=max_len, causal=bool(causal), q_pos0=q_pos0, window=window)
+    return Kv4AttnParams(*ints, float(scale if scale is not None else 1.0 / math.sqrt(D)), float(softcap), int(o_fmt))
 
 
 def kv4_attention_plan(p):
@@ -608,19 +633,22 @@ def kv4_attention_plan(p):
 def kv4_attention(p, q, cache, kv_len=None, out=None, workspace=None, stream=None):
     """O of new queries over a Kv4Cache (mxfa_kv4_attention): q bfloat16 [B, Hq, Sq, D] and out [B, Hq, Sq, D] of
     p.o_fmt, rows contiguous, the other strides free; kv_len: int32 CUDA tensor [B], each sequence's keys
-    (None: p.seq_k, queries from p.q_pos0 on).  workspace: a uint8 tensor of kv4_attention_plan's bytes."""
+    (None: p.seq_k, queries from p.q_pos0 on).  workspace: a uint8 tensor of kv4_attention_plan's bytes, one for each
+    of the calls that may overlap (None allocates)."""
     c, dev = cache.shape, cache.k.device
     if (p.batch, p.num_kv_heads, p.head_dim, p.max_len) != (c.batch, c.num_kv_heads, c.head_dim, c.max_len):
         raise MxfaError(1, "the parameters' batch, num_kv_heads, head_dim and max_len are not the cache's")
     shape = (p.batch, p.num_q_heads, p.seq_q, p.head_dim)
     dtype = torch.bfloat16 if p.o_fmt == C_BF16 else torch.float32
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=dev)
+        out = _empty(shape, dtype, dev, stream)
     qs, os_ = _rows(q, torch.bfloat16, shape, dev, "q"), _rows(out, dtype, shape, dev, "out", True)
     _on(dev)
     if workspace is None:
-        workspace = torch.empty(kv4_attention_plan(p)[1], dtype=torch.uint8, device=dev)
+        workspace = _empty(kv4_attention_plan(p)[1], torch.uint8, dev, stream)
     _need(workspace, torch.uint8, (workspace.numel(),), "workspace")
+    if workspace.get_device() != dev.index:
+        raise MxfaError(1, f"workspace must be on {dev}")
     _check(lib().mxfa_kv4_attention(p, q.data_ptr(), qs, cache.k.data_ptr(), cache.ks.data_ptr(), cache.v.data_ptr(),
                                     cache.vs.data_ptr(), _index(kv_len, p.batch, dev, "kv_len"), out.data_ptr(), os_,
                                     workspace.data_ptr(), workspace.numel(), _stream(stream)))
@@ -644,14 +672,14 @@ def rmsnorm_quantize(x, weight, eps=1e-6, residual=None, weight_offset=0.0, gemm
     else:
         _need(residual, x.dtype, x.shape, "residual")
         if h is None:
-            h = torch.empty_like(x)
+            h = _empty(x.shape, x.dtype, dev, stream)
         _need(h, x.dtype, x.shape, "h")
     for t, name in ((weight, "weight"), (residual, "residual"), (h, "h")):
         if t is not None and t.get_device() != dev.index:
             raise MxfaError(1, f"{name} must be on {dev}")
     _on(dev)
-    codes = torch.empty_like(x, dtype=torch.uint8)
-    scales = torch.empty((cols // 32, rows) if gemm_scales else (*x.shape[:-1], cols // 32), dtype=torch.uint8, device=dev)
+    codes = _empty(x.shape, torch.uint8, dev, stream)
+    scales = _empty((cols // 32, rows) if gemm_scales else (*x.shape[:-1], cols // 32), torch.uint8, dev, stream)
     p = NormParams(rows, cols, fmt, float(eps), float(weight_offset), rows if gemm_scales else 0)
     _check(lib().mxfa_rmsnorm_quantize(p, x.data_ptr(), _ptr(residual), weight.data_ptr(), _ptr(h),
                                        codes.data_ptr(), scales.data_ptr(), _stream(stream)))

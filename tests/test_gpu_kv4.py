@@ -460,6 +460,39 @@ def test_refusals_of_tensors():
     assert cache.length == 0 and not bool(cache.k.any())
 
 
+def test_refusals_of_places_and_counts():
+    cache = mxfa.Kv4Cache(2, 2, 128, 64)
+    x = torch.zeros((2, 2, 3, 128), device=DEV)
+    for f in (lambda: cache.append(x, x, counts=torch.ones(2, dtype=torch.int32, device=DEV)),   # (no common length then)
+              lambda: cache.read(3, pos=1 << 32), lambda: cache.read(-1), lambda: cache.read((1 << 32) + 1),
+              lambda: mxfa.Kv4Cache.of(cache.k[0], cache.ks, cache.v, cache.vs), lambda: mxfa.Kv4Cache.of(None, None, None, None)):
+        with pytest.raises(mxfa.MxfaError):
+            f()
+    assert cache.length == 0
+
+
+def test_what_a_call_allocates_belongs_to_its_stream(monkeypatch):
+    """Outputs and workspaces come from the stream that the call runs on, handle or object."""
+    q, cache, lt = _problem(1, 8, 2, 1, 128, 4128, [4096], seed=3)
+    p = mxfa.make_kv4_params(1, 8, 2, 1, 4096, 128, 4128)
+    assert mxfa.kv4_attention_plan(p)[1] > 0
+    w = torch.ones(128, device=DEV)
+    x = torch.randn((5, 128), device=DEV)
+    calls = [lambda s: mxfa.kv4_attention(p, q, cache, kv_len=lt, stream=s), lambda s: cache.read(7, stream=s)[0],
+             lambda s: mxfa.rmsnorm_quantize(x, w, residual=x, stream=s)[0]]
+    want = [f(None) for f in calls]
+    torch.cuda.synchronize()
+    side, seen, empty = torch.cuda.Stream(), [], torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: (seen.append(torch.cuda.current_stream().cuda_stream), empty(*a, **k))[1])
+    for f, y in zip(calls, want):
+        for s in (side, side.cuda_stream):
+            seen.clear()
+            got = f(s)
+            assert seen and set(seen) == {side.cuda_stream}
+            side.synchronize()
+            assert torch.equal(got, y)
+
+
 def test_graph_and_streams():
     """A decode step over device-side lengths, captured once and replayed while the lengths grow, with eager calls
     of the same kind on another stream in between, equals the eager steps."""

@@ -128,3 +128,17 @@ def test_reference_rule_on_the_values_themselves():
     assert sorted(R.scale_place(t, b, 4).ravel()) == list(range(256))
     by = np.random.default_rng(0).integers(0, 256, (1, 2, 64, 4)).astype(np.uint8)
     assert np.array_equal(R.scales_by_token(R.scales_in_cache(by)), by)
+
+
+def test_values_past_32_bits_are_refused_not_cut():
+    for kw in (dict(window=1 << 32), dict(q_pos0=1 << 32), dict(Sk=1 << 32), dict(max_len=(1 << 32) + 256), dict(B=(1 << 32) + 1)):
+        with pytest.raises(mxfa.MxfaError, match="32 bits"):
+            _params(**kw)
+    for args in ((0, 1, 64, 32), (1, 1, 48, 32), (1, 1, 64, 33), (1, 1, 64, 0), (1, 1, 64, (1 << 32) + 32)):
+        with pytest.raises(mxfa.MxfaError):
+            mxfa.Kv4Cache(*args, device="cpu")
+
+
+def test_scales_that_leave_the_float_range_are_refused():
+    for kw in (dict(scale=3e38), dict(softcap=3e38), dict(softcap=1e-42)):
+        assert _attend(_params(**kw)) == 1 and "log2 units" in _err(), kw
