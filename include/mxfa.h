@@ -380,8 +380,10 @@ typedef struct {
 
 /* The norm in front of a projection, to the operand that mxfa_gemm takes: h = x + residual, rounded to
  * x_fmt and written to h (residual NULL: h = x, and h may be NULL), y = h / sqrt(mean(h^2) + eps) * (weight +
- * weight_offset) in fp32, y to E4M3 codes [rows][cols] and scales by rule R1 (the codes of
- * mxfa_quantize_rows).  x, residual, h [rows][cols]; h may be x or residual (the same tensor, in place). */
+ * weight_offset), y to E4M3 codes [rows][cols] and scales by rule R1 (the codes of
+ * mxfa_quantize_rows).  The sum of squares is fp32 per thread and 64 bits across, and y is rounded to odd, so
+ * codes and scales are those of y itself, not of its nearest fp32 value.  x, residual, h [rows][cols]; h
+ * may be x or residual (the same tensor, in place). */
 mxfa_status mxfa_rmsnorm_quantize(const mxfa_norm_params *p, const void *x, const void *residual, const void *weight,
                                   void *h, uint8_t *codes, uint8_t *scales, void *stream);
 

@@ -135,3 +135,16 @@ def test_norm_refusals():
             f()
     codes, scales, h = mxfa.rmsnorm_quantize(x[:0], w, gemm_scales=True)
     assert codes.shape == (0, 64) and scales.shape == (2, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_just_below_a_power_of_two(dtype):
+    """y = 4 (1 - 5e-9) lies below 4, though nearest to it in 32 bits: the block's scale is that of the values from 2 on,
+    2^(1 - 8), under which y saturates at 448.  And y = 17/16 (1 - 5e-9), just below a tie of two codes, takes the
+    lower one."""
+    w = torch.full((128,), 4.0, dtype=dtype, device=DEV)
+    w[64:] = 17 / 16
+    codes, scales, _ = mxfa.rmsnorm_quantize(torch.ones((3, 128), dtype=dtype, device=DEV), w, eps=1e-8)
+    assert scales.cpu().tolist() == [[120, 120, 119, 119]] * 3
+    got = codes.view(torch.float8_e4m3fn).float().cpu()
+    assert bool((got[:, :64] == 448).all()) and bool((got[:, 64:] == 256).all())
